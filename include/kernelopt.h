@@ -50,6 +50,15 @@ typedef struct CUstream_st* ko_stream_t; /* identical to cudaStream_t */
 #define KO_ACT_RELU 2
 #define KO_ACT_SILU 3 /* v / (1 + exp(-v)); ko_layernorm only */
 
+/* Element types of the entry points that take more than float32. */
+#define KO_F32 0
+#define KO_BF16 1
+#define KO_F16 2
+
+/* Microscaled formats (OCP MX): 32 consecutive elements along K share one e8m0 scale (a power of two). */
+#define KO_MXFP4 0 /* e2m1 elements, two per byte: +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} */
+#define KO_MXFP8 1 /* e4m3 elements, one per byte: up to +-448 */
+
 /* --- status / version ------------------------------------------------------------------------------------- */
 
 /* Text of the last failure on the calling host thread ("" if none). */
@@ -289,6 +298,50 @@ int ko_linear_small_f32(const float* x, const float* w, const float* bias, int64
  * 16-byte aligned, K <= 3072. Replaces bbox_embed's last layer and the box arithmetic of fast_rfdetr/model.py:270-272. */
 int ko_box_head_f32(const float* x, const float* w, const float* bias, const float* ref, int64_t M, int64_t K,
                     float* boxes, ko_stream_t stream);
+
+/* --- microscaled (MX) quantisation, norm and products --------------------------------------------------------- */
+
+/* A matrix [rows][K] in an MX format, with Kp = K rounded up to a multiple of 128:
+ *   codes:  KO_MXFP4 [rows][Kp / 2] bytes, element 2i in the low nibble of byte i; KO_MXFP8 [rows][Kp] bytes
+ *   scales: [ceil(rows / 128)][Kp / 128][32][4][4] e8m0 bytes: that of row 128 R + 32 j + i and block 4 T + b (of 32
+ *           elements) is byte (i, j, b) of tile (R, T)
+ * What fills up K (zero codes, scale byte 0) and the scales of rows up to a multiple of 128 (byte 0) is written too.
+ * Element k of a row stands for code * 2^(byte - 127). A block's byte is floor(log2(max |v|)) - emax + 127, held to 0
+ * or above, with emax 2 (MXFP4) or 8 (MXFP8); its codes are v / 2^(byte - 127) to nearest even, saturating at the
+ * largest element. A block that holds a NaN or an infinity gets byte 255 (NaN) and zero codes. Both buffers are 16-byte
+ * aligned. The reference has no reduced-precision path: no counterpart there. */
+int64_t ko_mx_codes_bytes(int64_t rows, int64_t K, int fmt); /* -1 for a bad size or format */
+int64_t ko_mx_scales_bytes(int64_t rows, int64_t K);         /* -1 for a bad size */
+
+/* x: [rows][K] of `dtype` (KO_F32 / KO_BF16 / KO_F16), row r at x + r * ldx elements -> codes, scales in `fmt`. */
+int ko_quantize_mx(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, int fmt, void* codes, void* scales,
+                   ko_stream_t stream);
+
+/* The values that codes and scales stand for, rounded once to `dtype`: out [rows][K], contiguous. */
+int ko_dequantize_mx(const void* codes, const void* scales, int fmt, int64_t rows, int64_t K, void* out, int dtype,
+                     ko_stream_t stream);
+
+/* A weight w: [K][N] of `dtype` (the x @ W convention, contiguous) -> its transpose [N][K] in KO_MXFP4, blocks along K.
+ * Run once per weight; the result feeds ko_linear_mxfp4. */
+int ko_pack_weight_mxfp4(const void* w, int dtype, int64_t K, int64_t N, void* codes, void* scales,
+                         ko_stream_t stream);
+
+/* v = h + (o + bias) * scale;  y = v / sqrt(mean(v^2) + eps) * gamma over rows of C (statistics and y in fp32 from the
+ * unrounded v). h, o: [rows][C] of `dtype`, rows ldh / ldo elements apart; bias, scale, gamma: [C] of `dtype`; o NULL
+ * = no residual (bias and scale then unused), bias / scale NULL = 0 / 1. h_out: [rows][C] receives v rounded to
+ * `dtype`, or NULL; it may be h itself when ldh == C. Exactly one form of y: y [rows][C] of `dtype`, or y NULL and
+ * codes, scales in `fmt`. 1 <= C <= 32768. Stands beside ko_residual_layernorm for models that normalise by the root
+ * mean square. */
+int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, int64_t ldo, const void* bias, const void* scale,
+                        const void* gamma, int dtype, float eps, int64_t rows, int64_t C, void* h_out, void* y, int fmt,
+                        void* codes, void* scales, ko_stream_t stream);
+
+/* out = act(A @ W^T + bias): A [M][K] in a_fmt (KO_MXFP4 or KO_MXFP8), W [N][K] in KO_MXFP4 (ko_pack_weight_mxfp4),
+ * bias float32 [N] or NULL, fp32 accumulation, act KO_ACT_NONE, KO_ACT_GELU (erf form) or KO_ACT_RELU, out [M][N] of
+ * `out_dtype`, contiguous. Codes and scales as above; dev_status as for ko_linear_f32_packed. */
+int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_fmt, const void* w_codes, const void* w_scales,
+                    const float* bias, int64_t M, int64_t K, int64_t N, int act, void* out, int out_dtype,
+                    int* dev_status, ko_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,414 @@
+// Microscaled quantisation, its inverse, the 4-bit weight layout, and the residual + root-mean-square norm whose output
+// can be microscaled in the same pass. Formats and layout: ko_mx.cuh.
+//
+// All of these read and write each byte once and compute a few operations per element, so HBM bounds them. Eight
+// consecutive elements belong to a lane, four lanes to a block of 32 and sixteen lanes to the 128 elements of a scale
+// word, so a block's largest magnitude is two shuffles and its four scales are written as one 32-bit word.
+#include <cmath>
+#include <string>
+
+#include "ko_mx.cuh"
+
+namespace {
+
+using namespace komx;
+
+constexpr int kThreads = 256;
+
+// ---------------------------------------------------------------------------------------------------------
+// Quantisation: half a warp takes the 128 elements of one scale word at a time. Items run over k tiles, then rows,
+// the rows that fill the last tile of 128 included (scale words 0, no codes).
+// ---------------------------------------------------------------------------------------------------------
+template <typename T, int FMT, bool VEC>
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t K,
+                                                            int64_t ldx, int64_t items, uint32_t ktiles,
+                                                            int64_t code_pitch, uint8_t* __restrict__ codes,
+                                                            uint8_t* __restrict__ scales) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
+  if (item >= items) return;
+  const int64_t row = items <= 0xffffffffll ? static_cast<uint32_t>(item) / ktiles : item / ktiles;
+  const int64_t kt = item - row * ktiles;
+  uint8_t* word = scales + scale_word_offset(row, kt, ktiles);
+  if (row >= rows) {
+    if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(word) = 0u;
+    return;
+  }
+  float v[8];
+  load8<T, VEC>(x + row * ldx, kt * 128 + (threadIdx.x & 15) * 8, K, v);
+  quantize_group<FMT>(v, 0xffffu << (threadIdx.x & 16), codes + row * code_pitch, kt, word);
+}
+
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
+                                                              const uint8_t* __restrict__ scales, int64_t K,
+                                                              int64_t items, uint32_t ktiles, int64_t code_pitch,
+                                                              T* __restrict__ out, bool vec) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
+  if (item >= items) return;
+  const int64_t row = items <= 0xffffffffll ? static_cast<uint32_t>(item) / ktiles : item / ktiles;
+  const int64_t kt = item - row * ktiles;
+  const int lane16 = threadIdx.x & 15;
+  const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(scales + scale_word_offset(row, kt, ktiles)));
+  const float s = scale_value((word >> (8 * (lane16 >> 2))) & 255u);
+  const uint8_t* src = codes + row * code_pitch;
+  float v[8];
+  if constexpr (FMT == KO_MXFP4) {
+    unpack_e2m1x8(__ldg(reinterpret_cast<const uint32_t*>(src + kt * 64 + lane16 * 4)), v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= s;
+  } else {
+    const uint2 c = __ldg(reinterpret_cast<const uint2*>(src + kt * 128 + lane16 * 8));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack_e4m3x2(((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xffffu);
+      v[2 * i] = f.x * s;
+      v[2 * i + 1] = f.y * s;
+    }
+  }
+  T* dst = out + row * K;
+  const int64_t c0 = kt * 128 + lane16 * 8;
+  if (vec) store8<T, true>(dst, c0, K, v);
+  else store8<T, false>(dst, c0, K, v);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// A weight [K][N] to its transpose in mxfp4: a thread takes one column of 32 rows, a whole block. Neighbouring threads
+// read neighbouring columns; each writes the block's 16 bytes. Once per weight, so the scattered writes stay.
+// ---------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pack_weight_kernel(const T* __restrict__ w, int64_t K, int64_t N,
+                                                               uint32_t kblocks, int64_t n_blocks,
+                                                               int64_t code_pitch, uint8_t* __restrict__ codes,
+                                                               uint8_t* __restrict__ scales) {
+  const int64_t kb = blockIdx.x % kblocks;
+  const int64_t n = static_cast<int64_t>(blockIdx.x / kblocks) * kThreads + threadIdx.x;
+  if (n >= n_blocks) return;  // n_blocks: N rounded up to the scale tile's 128
+  uint8_t* byte_at = scales + scale_word_offset(n, kb >> 2, kblocks >> 2) + (kb & 3);
+  if (n >= N) {
+    *byte_at = 0;
+    return;
+  }
+  float v[32];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int64_t k = kb * 32 + i;
+    v[i] = k < K ? to_f(w[k * N + n]) : 0.f;
+    m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  const uint32_t byte = scale_byte<KO_MXFP4>(m);
+  const float inv = scale_inverse(byte);
+  uint32_t c[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = v[g * 8 + i];
+    c[g] = byte == 255u ? 0u : pack_e2m1x8(t, inv);
+  }
+  *byte_at = static_cast<uint8_t>(byte);
+  *reinterpret_cast<uint4*>(codes + n * code_pitch + kb * 16) = make_uint4(c[0], c[1], c[2], c[3]);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Residual + root-mean-square norm. T threads share a row and keep its NV groups of eight elements each in fp32
+// registers from the load to the store, so h and o are read once; the sum of squares is a shuffle tree and, for rows of
+// more than a warp, one exchange through shared memory, both in a fixed order. OUT: -1 writes y in the input's type, else
+// the MX format.
+// ---------------------------------------------------------------------------------------------------------
+struct NormArgs {
+  const void *h, *o, *bias, *scale, *gamma;
+  void *h_out, *y;
+  uint8_t *codes, *scales;
+  int64_t ldh, ldo, rows, C, code_pitch, grid_rows;
+  uint32_t ktiles;
+  float eps;
+};
+
+template <typename T, int OUT, bool VEC, int TPR, int NV>
+__global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kernel(const NormArgs a) {
+  constexpr int kBlock = TPR > kThreads ? TPR : kThreads;
+  constexpr int kRows = kBlock / TPR;
+  constexpr int kWarps = TPR / 32;  // warps of a row (0: half a warp)
+  __shared__ float part[kBlock / 32];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+  const bool real = row < a.rows;
+  const int64_t C = a.C;
+  float v[NV][8];
+  float sum = 0.f;
+  if (real) {
+    const T* h = static_cast<const T*>(a.h) + row * a.ldh;
+    const T* o = a.o ? static_cast<const T*>(a.o) + row * a.ldo : nullptr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (t + i * TPR) * 8;
+      if (c >= C) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        continue;
+      }
+      load8<T, VEC>(h, c, C, v[i]);
+      if (o) {
+        float r[8];
+        load8<T, VEC>(o, c, C, r);
+        if (a.bias) {
+          float b[8];
+          load8<T, VEC>(static_cast<const T*>(a.bias), c, C, b);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) r[j] += b[j];
+        }
+        if (a.scale) {
+          float s[8];
+          load8<T, VEC>(static_cast<const T*>(a.scale), c, C, s);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) r[j] *= s[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += r[j];
+      }
+      if (a.h_out) store8<T, VEC>(static_cast<T*>(a.h_out) + row * C, c, C, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      sum += ((v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3])) +
+             ((v[i][4] * v[i][4] + v[i][5] * v[i][5]) + (v[i][6] * v[i][6] + v[i][7] * v[i][7]));
+  }
+#pragma unroll
+  for (int s = (TPR < 32 ? TPR : 32) / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  if constexpr (kWarps > 1) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    const int w0 = (threadIdx.x / TPR) * kWarps;
+    float p = (threadIdx.x & 31) < kWarps ? part[w0 + (threadIdx.x & 31)] : 0.f;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) p += __shfl_xor_sync(0xffffffffu, p, s);
+    sum = p;
+  }
+  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(C) + a.eps);
+  if (row >= a.grid_rows) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t g = t + i * TPR;
+    const int64_t c = g * 8;
+    if constexpr (OUT < 0) {
+      if (real && c < C) {
+        float gm[8];
+        load8<T, VEC>(static_cast<const T*>(a.gamma), c, C, gm);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * gm[j];
+        store8<T, VEC>(static_cast<T*>(a.y) + row * C, c, C, v[i]);
+      }
+    } else {
+      const int64_t kt = g >> 4;
+      if (kt < a.ktiles) {  // the same for the sixteen lanes of a group
+        uint8_t* word = a.scales + scale_word_offset(row, kt, a.ktiles);
+        if (!real) {
+          if ((t & 15) == 0) *reinterpret_cast<uint32_t*>(word) = 0u;
+        } else {
+          float gm[8];
+          load8<T, VEC>(static_cast<const T*>(a.gamma), c, C, gm);
+          // beyond C: v is 0 there and gm is 0; 0 * rstd would be NaN for an infinite rstd (eps 0, a row of zeros)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = c + j < C ? v[i][j] * rstd * gm[j] : 0.f;
+          quantize_group<OUT>(v[i], 0xffffu << (threadIdx.x & 16), a.codes + row * a.code_pitch, kt, word);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int OUT, bool VEC, int TPR, int NV>
+int launch_norm(const NormArgs& a, cudaStream_t s) {
+  constexpr int kBlock = TPR > kThreads ? TPR : kThreads;
+  const int64_t blocks = (a.grid_rows + kBlock / TPR - 1) / (kBlock / TPR);
+  if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_residual_rmsnorm: too many rows");
+  rmsnorm_kernel<T, OUT, VEC, TPR, NV><<<static_cast<unsigned>(blocks), kBlock, 0, s>>>(a);
+  return ko::check_launch("ko_residual_rmsnorm");
+}
+
+template <typename T, int OUT, bool VEC>
+int pick_norm(const NormArgs& a, cudaStream_t s) {
+  if (a.C <= 384) return launch_norm<T, OUT, VEC, 16, 3>(a, s);
+  if (a.C <= 1024) return launch_norm<T, OUT, VEC, 32, 4>(a, s);
+  if (a.C <= 2048) return launch_norm<T, OUT, VEC, 64, 4>(a, s);
+  if (a.C <= 4096) return launch_norm<T, OUT, VEC, 128, 4>(a, s);
+  if (a.C <= 8192) return launch_norm<T, OUT, VEC, 256, 4>(a, s);
+  if (a.C <= 16384) return launch_norm<T, OUT, VEC, 512, 4>(a, s);
+  return launch_norm<T, OUT, VEC, 1024, 4>(a, s);
+}
+
+template <typename T>
+int dispatch_norm(const NormArgs& a, int out, bool vec, cudaStream_t s) {
+  if (out < 0) return vec ? pick_norm<T, -1, true>(a, s) : pick_norm<T, -1, false>(a, s);
+  if (out == KO_MXFP4) return vec ? pick_norm<T, KO_MXFP4, true>(a, s) : pick_norm<T, KO_MXFP4, false>(a, s);
+  return vec ? pick_norm<T, KO_MXFP8, true>(a, s) : pick_norm<T, KO_MXFP8, false>(a, s);
+}
+
+template <typename T, int FMT>
+int launch_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, void* codes, void* scales, bool vec,
+                    cudaStream_t s) {
+  const int64_t ktiles = padded_k(K) / 128, items = (rows + 127) / 128 * 128 * ktiles;
+  const int64_t blocks = (items + kThreads / 16 - 1) / (kThreads / 16);
+  if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_quantize_mx: too many elements");
+  const int64_t pitch = code_pitch(K, FMT);
+  uint8_t *c = static_cast<uint8_t*>(codes), *sc = static_cast<uint8_t*>(scales);
+  const unsigned g = static_cast<unsigned>(blocks);
+  if (vec)
+    quantize_kernel<T, FMT, true><<<g, kThreads, 0, s>>>(static_cast<const T*>(x), rows, K, ldx, items,
+                                                         static_cast<uint32_t>(ktiles), pitch, c, sc);
+  else
+    quantize_kernel<T, FMT, false><<<g, kThreads, 0, s>>>(static_cast<const T*>(x), rows, K, ldx, items,
+                                                          static_cast<uint32_t>(ktiles), pitch, c, sc);
+  return ko::check_launch("ko_quantize_mx");
+}
+
+template <typename T>
+int launch_dequantize(const void* codes, const void* scales, int fmt, int64_t rows, int64_t K, void* out,
+                      cudaStream_t s) {
+  const int64_t ktiles = padded_k(K) / 128, items = rows * ktiles;
+  const int64_t blocks = (items + kThreads / 16 - 1) / (kThreads / 16);
+  if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_dequantize_mx: too many elements");
+  const bool vec = ko::aligned16(out) && (K * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+  const uint8_t *c = static_cast<const uint8_t*>(codes), *sc = static_cast<const uint8_t*>(scales);
+  const unsigned g = static_cast<unsigned>(blocks);
+  if (fmt == KO_MXFP4)
+    dequantize_kernel<T, KO_MXFP4><<<g, kThreads, 0, s>>>(c, sc, K, items, static_cast<uint32_t>(ktiles),
+                                                          code_pitch(K, fmt), static_cast<T*>(out), vec);
+  else
+    dequantize_kernel<T, KO_MXFP8><<<g, kThreads, 0, s>>>(c, sc, K, items, static_cast<uint32_t>(ktiles),
+                                                          code_pitch(K, fmt), static_cast<T*>(out), vec);
+  return ko::check_launch("ko_dequantize_mx");
+}
+
+bool aligned_to(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(n) == 0; }
+
+}  // namespace
+
+extern "C" int64_t ko_mx_codes_bytes(int64_t rows, int64_t K, int fmt) {
+  if (rows < 0 || rows > kMaxRows || K < 1 || K > kMaxK || !fmt_ok(fmt)) return -1;
+  return rows * code_pitch(K, fmt);
+}
+extern "C" int64_t ko_mx_scales_bytes(int64_t rows, int64_t K) {
+  if (rows < 0 || rows > kMaxRows || K < 1 || K > kMaxK) return -1;
+  return (rows + 127) / 128 * 128 * (padded_k(K) / 32);
+}
+
+extern "C" int ko_quantize_mx(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, int fmt, void* codes,
+                              void* scales, ko_stream_t stream) {
+  const std::string who = "ko_quantize_mx: ";
+  if (rows < 0 || rows > kMaxRows || K < 1 || K > kMaxK || ldx < K)
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "need 0 <= rows <= 2^31, 1 <= K <= 2^24 and ldx >= K");
+  if (!dtype_ok(dtype) || !fmt_ok(fmt)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "unknown element type or format");
+  if (rows == 0) return KO_OK;
+  if (!x || !codes || !scales) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
+  const int64_t es = dtype_size(dtype);
+  if (!aligned_to(x, es) || !ko::aligned16(codes) || !ko::aligned16(scales))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "x must be aligned to its elements, codes and scales to 16 bytes");
+  const bool vec = ko::aligned16(x) && ldx * es % 16 == 0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool f4 = fmt == KO_MXFP4;
+  if (dtype == KO_F32)
+    return f4 ? launch_quantize<float, KO_MXFP4>(x, rows, K, ldx, codes, scales, vec, s)
+              : launch_quantize<float, KO_MXFP8>(x, rows, K, ldx, codes, scales, vec, s);
+  if (dtype == KO_BF16)
+    return f4 ? launch_quantize<__nv_bfloat16, KO_MXFP4>(x, rows, K, ldx, codes, scales, vec, s)
+              : launch_quantize<__nv_bfloat16, KO_MXFP8>(x, rows, K, ldx, codes, scales, vec, s);
+  return f4 ? launch_quantize<__half, KO_MXFP4>(x, rows, K, ldx, codes, scales, vec, s)
+            : launch_quantize<__half, KO_MXFP8>(x, rows, K, ldx, codes, scales, vec, s);
+}
+
+extern "C" int ko_dequantize_mx(const void* codes, const void* scales, int fmt, int64_t rows, int64_t K, void* out,
+                                int dtype, ko_stream_t stream) {
+  const std::string who = "ko_dequantize_mx: ";
+  if (rows < 0 || rows > kMaxRows || K < 1 || K > kMaxK)
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "need 0 <= rows <= 2^31 and 1 <= K <= 2^24");
+  if (!dtype_ok(dtype) || !fmt_ok(fmt)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "unknown element type or format");
+  if (rows == 0) return KO_OK;
+  if (!codes || !scales || !out) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
+  if (!ko::aligned16(codes) || !ko::aligned16(scales) || !aligned_to(out, dtype_size(dtype)))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "codes and scales must be 16-byte aligned, out to its elements");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == KO_F32) return launch_dequantize<float>(codes, scales, fmt, rows, K, out, s);
+  if (dtype == KO_BF16) return launch_dequantize<__nv_bfloat16>(codes, scales, fmt, rows, K, out, s);
+  return launch_dequantize<__half>(codes, scales, fmt, rows, K, out, s);
+}
+
+extern "C" int ko_pack_weight_mxfp4(const void* w, int dtype, int64_t K, int64_t N, void* codes, void* scales,
+                                    ko_stream_t stream) {
+  const std::string who = "ko_pack_weight_mxfp4: ";
+  if (K < 1 || K > kMaxK || N < 1 || N > kMaxRows)
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "need 1 <= K <= 2^24 and 1 <= N <= 2^31");
+  if (!dtype_ok(dtype)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "unknown element type");
+  if (!w || !codes || !scales) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
+  if (!aligned_to(w, dtype_size(dtype)) || !ko::aligned16(codes) || !ko::aligned16(scales))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "w must be aligned to its elements, codes and scales to 16 bytes");
+  const int64_t kblocks = padded_k(K) / 32, n_rows = (N + 127) / 128 * 128;
+  const int64_t blocks = kblocks * ((n_rows + kThreads - 1) / kThreads);
+  if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "the weight is too large");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const unsigned g = static_cast<unsigned>(blocks);
+  uint8_t *c = static_cast<uint8_t*>(codes), *sc = static_cast<uint8_t*>(scales);
+  const int64_t pitch = code_pitch(K, KO_MXFP4);
+  const uint32_t kb = static_cast<uint32_t>(kblocks);
+  if (dtype == KO_F32)
+    pack_weight_kernel<float><<<g, kThreads, 0, s>>>(static_cast<const float*>(w), K, N, kb, n_rows, pitch, c, sc);
+  else if (dtype == KO_BF16)
+    pack_weight_kernel<__nv_bfloat16><<<g, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(w), K, N, kb, n_rows,
+                                                             pitch, c, sc);
+  else
+    pack_weight_kernel<__half><<<g, kThreads, 0, s>>>(static_cast<const __half*>(w), K, N, kb, n_rows, pitch, c, sc);
+  return ko::check_launch("ko_pack_weight_mxfp4");
+}
+
+extern "C" int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, int64_t ldo, const void* bias,
+                                   const void* scale, const void* gamma, int dtype, float eps, int64_t rows,
+                                   int64_t C, void* h_out, void* y, int fmt, void* codes, void* scales,
+                                   ko_stream_t stream) {
+  const std::string who = "ko_residual_rmsnorm: ";
+  if (rows < 0 || rows > kMaxRows || C < 1 || C > 32768 || ldh < C || (o && ldo < C))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "need 0 <= rows <= 2^31, 1 <= C <= 32768 and pitches of at least C");
+  if (!dtype_ok(dtype)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "unknown element type");
+  if (!(eps >= 0.f)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "eps must not be negative");
+  if (y ? (codes || scales) : (!codes || !scales || !fmt_ok(fmt)))
+    if (rows > 0 || (y && (codes || scales)))
+      return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "give either y, or codes and scales with a known format");
+  if (rows == 0) return KO_OK;
+  if (!h || !gamma) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
+  if (!o && (bias || scale))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "bias and scale belong to o");
+  if (h_out == h && ldh != C)
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "h_out may be h only where h is contiguous");
+  const int64_t es = dtype_size(dtype);
+  bool vec = ldh * es % 16 == 0 && (!o || ldo * es % 16 == 0) && C * es % 16 == 0;
+  const void* elems[] = {h, o, bias, scale, gamma, h_out, y};
+  for (const void* p : elems) {
+    if (p && !aligned_to(p, es)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "a pointer is not aligned to its elements");
+    vec = vec && ko::aligned16(p);
+  }
+  if (!y && (!ko::aligned16(codes) || !ko::aligned16(scales)))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "codes and scales must be 16-byte aligned");
+  NormArgs a{};
+  a.h = h;
+  a.o = o;
+  a.bias = bias;
+  a.scale = scale;
+  a.gamma = gamma;
+  a.h_out = h_out;
+  a.y = y;
+  a.codes = static_cast<uint8_t*>(codes);
+  a.scales = static_cast<uint8_t*>(scales);
+  a.ldh = ldh;
+  a.ldo = ldo;
+  a.rows = rows;
+  a.C = C;
+  a.code_pitch = y ? 0 : code_pitch(C, fmt);
+  a.grid_rows = y ? rows : (rows + 127) / 128 * 128;
+  a.ktiles = static_cast<uint32_t>(padded_k(C) / 128);
+  a.eps = eps;
+  const int out = y ? -1 : fmt;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == KO_F32) return dispatch_norm<float>(a, out, vec, s);
+  if (dtype == KO_BF16) return dispatch_norm<__nv_bfloat16>(a, out, vec, s);
+  return dispatch_norm<__half>(a, out, vec, s);
+}

@@ -1,0 +1,221 @@
+// Microscaled (OCP MX) data as the library lays it out, and the conversions its kernels share.
+//
+// A matrix [rows][K] in an MX format is, with Kp = K rounded up to a multiple of 128:
+//   codes   mxfp4: [rows][Kp / 2] bytes, element 2i in the low nibble of byte i;  mxfp8: [rows][Kp] bytes
+//   scales  [ceil(rows / 128)][Kp / 128][32][4][4] bytes: the e8m0 scale of row 128 R + 32 j + i and block 4 T + b is
+//           byte (i, j, b) of tile (R, T). One tile is the 512 contiguous bytes that the block-scaled tensor-core
+//           products take as one operand: 32 tensor-memory lanes of 16 bytes, one 32-bit column per group of 32 rows.
+// Codes and scales beyond K are zero (scale byte 0, 2^-127), and so are the scales of the rows that fill the last tile.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ko_common.cuh"
+
+namespace komx {
+
+inline int64_t padded_k(int64_t K) { return (K + 127) / 128 * 128; }
+inline int64_t code_pitch(int64_t K, int fmt) { return fmt == KO_MXFP4 ? padded_k(K) / 2 : padded_k(K); }
+inline bool fmt_ok(int fmt) { return fmt == KO_MXFP4 || fmt == KO_MXFP8; }
+inline bool dtype_ok(int dt) { return dt == KO_F32 || dt == KO_BF16 || dt == KO_F16; }
+inline int64_t dtype_size(int dt) { return dt == KO_F32 ? 4 : 2; }
+// Bounds that keep every size and offset product of these entry points inside 62 bits.
+constexpr int64_t kMaxRows = int64_t(1) << 31;
+constexpr int64_t kMaxK = int64_t(1) << 24;
+
+#if defined(__CUDACC__)
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+// One rounding (to nearest even) from fp32 to the output's type.
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// Eight consecutive elements: 32 aligned bytes (fp32) or 16 (bf16, fp16).
+template <typename T> struct Vec8;
+template <> struct Vec8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    a = make_float4(v[0], v[1], v[2], v[3]);
+    b = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
+template <> struct __align__(16) Vec8<__nv_bfloat16> {
+  __nv_bfloat162 p[4];
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __bfloat1622float2(p[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  }
+};
+template <> struct __align__(16) Vec8<__half> {
+  __half2 p[4];
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(p[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  }
+};
+
+// Elements [c, c + 8) of a row of C, zero beyond C. VEC: the row starts on 16 bytes, so a whole group is one or two
+// 128-bit loads; otherwise, and in the group that C cuts, element by element.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t C, float (&v)[8]) {
+  if (VEC && c + 8 <= C) {
+    Vec8<T> t = *reinterpret_cast<const Vec8<T>*>(row + c);
+    t.get(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < C ? to_f(row[c + i]) : 0.f;
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* row, int64_t c, int64_t C, const float (&v)[8]) {
+  if (VEC && c + 8 <= C) {
+    Vec8<T> t;
+    t.set(v);
+    *reinterpret_cast<Vec8<T>*>(row + c) = t;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < C) row[c + i] = from_f<T>(v[i]);
+  }
+}
+
+// Largest magnitude of eight values as the bits of an fp32: ordered like the magnitudes, with infinity and then NaN
+// above every finite value, so that one integer maximum also finds what is not finite.
+__device__ __forceinline__ uint32_t amax_bits8(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+// The block's e8m0 byte: floor(log2(amax)) - emax + 127, held to 0 or above; 255 (NaN) where amax is not finite. The
+// exponent field of amax is floor(log2) + 127 for a normal number, and both subnormals and zero end at byte 0.
+template <int FMT>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
+  constexpr int emax = FMT == KO_MXFP4 ? 2 : 8;
+  const int e = static_cast<int>(amax_bits >> 23);
+  return e == 255 ? 255u : static_cast<uint32_t>(max(e - emax, 0));
+}
+// 2^(127 - byte), the exact reciprocal of the scale (byte <= 252 where it is not NaN); 0 for a NaN scale, whose block
+// holds zero codes.
+__device__ __forceinline__ float scale_inverse(uint32_t byte) {
+  return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+}
+// 2^(byte - 127); byte 0 is the subnormal 2^-127, byte 255 NaN.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return byte == 0u ? __uint_as_float(0x00400000u) : byte == 255u ? __uint_as_float(0x7fc00000u)
+                                                                  : __uint_as_float(byte << 23);
+}
+
+// Eight scaled values to e2m1 codes (element 0 in the lowest nibble), to nearest even, saturating at 6.
+__device__ __forceinline__ uint32_t pack_e2m1x8(const float (&v)[8], float inv) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
+        "f"(v[6] * inv), "f"(v[7] * inv));
+  return r;
+}
+// Eight scaled values to e4m3 codes, to nearest even, saturating at 448.
+__device__ __forceinline__ uint2 pack_e4m3x8(const float (&v)[8], float inv) {
+  uint2 r;
+  asm("{\n\t.reg .b16 h0, h1, h2, h3;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 h0, %3, %2;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 h1, %5, %4;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 h2, %7, %6;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 h3, %9, %8;\n\t"
+      "mov.b32 %0, {h0, h1};\n\tmov.b32 %1, {h2, h3};\n\t}"
+      : "=r"(r.x), "=r"(r.y)
+      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
+        "f"(v[6] * inv), "f"(v[7] * inv));
+  return r;
+}
+// Eight e2m1 codes as fp32 (exact in fp16 on the way). The bytes are taken apart inside the asm, from a whole 32-bit word:
+// fed from an 8-bit load, the conversion came out as zeros (CUDA 12.9).
+__device__ __forceinline__ void unpack_e2m1x8(uint32_t w, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+// Two e4m3 codes of a half word as fp32.
+__device__ __forceinline__ float2 unpack_e4m3x2(uint32_t half_word) {
+  uint32_t h;
+  asm("{\n\t.reg .b16 b;\n\tcvt.u16.u32 b, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(h) : "r"(half_word));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+
+// Byte offset of the scale word (the four scales of 128 elements) of (row, k tile).
+__device__ __forceinline__ int64_t scale_word_offset(int64_t row, int64_t ktile, int64_t ktiles) {
+  const int r = static_cast<int>(row & 127);
+  return ((row >> 7) * ktiles + ktile) * 512 + (r & 31) * 16 + (r >> 5) * 4;
+}
+
+// Writes the codes of a lane's eight values and, from one lane in sixteen, the scale word of their 128 elements.
+// Every group of sixteen lanes that calls this together holds one row's elements [128 kt, 128 kt + 128) in order;
+// `mask` names the calling lanes.
+template <int FMT>
+__device__ __forceinline__ void quantize_group(const float (&v)[8], uint32_t mask, uint8_t* __restrict__ code_row,
+                                               int64_t kt, uint8_t* __restrict__ scale_word) {
+  const int lane16 = threadIdx.x & 15;
+  uint32_t m = amax_bits8(v);
+  m = max(m, __shfl_xor_sync(mask, m, 1));
+  m = max(m, __shfl_xor_sync(mask, m, 2));
+  const uint32_t byte = scale_byte<FMT>(m);
+  const float inv = scale_inverse(byte);
+  if constexpr (FMT == KO_MXFP4) {
+    // a NaN or an infinity times the zero inverse is NaN, which would convert to the largest code
+    const uint32_t c = byte == 255u ? 0u : pack_e2m1x8(v, inv);
+    *reinterpret_cast<uint32_t*>(code_row + kt * 64 + lane16 * 4) = c;
+  } else {
+    uint2 c = pack_e4m3x8(v, inv);
+    if (byte == 255u) c = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(code_row + kt * 128 + lane16 * 8) = c;
+  }
+  uint32_t w = byte << (8 * (lane16 >> 2));
+  w |= __shfl_xor_sync(mask, w, 4);
+  w |= __shfl_xor_sync(mask, w, 8);
+  if (lane16 == 0) *reinterpret_cast<uint32_t*>(scale_word) = w;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace komx

@@ -15,6 +15,9 @@ pre-split weight form of the GEMM (`pack_weight` / `linear`) used for every dens
 LayerNorm epilogue (`linear_residual_layernorm`) and the implicit 3x3 convolution (`conv3x3_layernorm`);
 `layernorm`, `im2col3x3`; the backbone's `window_partition_layernorm` / `window_merge_layernorm`; the decoder's
 `select_queries` and `deform_prep`.
+And a microscaled (OCP MX) path, which the reference has no counterpart of: `quantize_mx`, `residual_rmsnorm` /
+`rmsnorm` with an mxfp8 or mxfp4 output, and `pack_weight_mxfp4` / `linear_mxfp4`. These take float32, bfloat16 and
+float16, any width and any even row pitch (column slices), and launch on the device of their tensors.
 """
 from __future__ import annotations
 
@@ -531,4 +534,224 @@ def linear_gelu_f32(x, w, bias):
     out = torch.empty((*x.shape[:-1], pw.n), dtype=torch.float32, device=x.device)
     call("ko_linear_f32_packed", x.data_ptr(), pw.packed.data_ptr(), bias.data_ptr(), m, pw.k, pw.n,
          _lib.KO_ACT_GELU, out.data_ptr(), status_word(x.device).data_ptr(), _stream())
+    return out
+
+
+# ---- microscaled (MX) formats ----
+MX_FORMATS = {"mxfp4": _lib.KO_MXFP4, "mxfp8": _lib.KO_MXFP8}
+MX_DTYPES = {torch.float32: _lib.KO_F32, torch.bfloat16: _lib.KO_BF16, torch.float16: _lib.KO_F16}
+
+
+def _call_on(device, name, *args):
+    """call(name, *args, stream) on the current stream of `device`, which need not be the current device."""
+    if device.index == torch.cuda.current_device():
+        return call(name, *args, torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        return call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _rows(t, name, dtype=None, device=None):
+    """(rows, elements between their starts) of t [..., width] with a contiguous last dimension and evenly spaced rows:
+    a dense tensor or a column slice of one."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.dtype not in MX_DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{name} must be [..., width] with width >= 1")
+    width = t.shape[-1]
+    rows = t.numel() // width
+    if t.is_contiguous() or rows == 0:
+        return rows, width
+    if width > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+    pitch = step = None
+    for d in range(t.dim() - 2, -1, -1):  # every leading dimension steps by whole rows
+        if t.shape[d] == 1:
+            continue
+        if pitch is None:
+            pitch = step = t.stride(d)
+        elif t.stride(d) != step:
+            raise ValueError(f"{name}: rows are not evenly spaced")
+        step *= t.shape[d]
+    if pitch is None:
+        return rows, width
+    if pitch < width:
+        raise ValueError(f"{name}: rows overlap (pitch {pitch}, width {width})")
+    return rows, pitch
+
+
+def _vector(t, name, width, dtype, device):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on {device}")
+    if t.dtype != dtype or t.numel() != width or not t.is_contiguous():
+        raise ValueError(f"{name} must hold {width} contiguous {dtype} elements")
+    return t.data_ptr()
+
+
+class MXTensor:
+    """A [..., K] tensor in a microscaled format: every 32 elements along K share a power of two.
+
+    fmt "mxfp4" (e2m1 elements) or "mxfp8" (e4m3); shape the logical shape; dtype the type it was made from. `codes`
+    is [rows, Kp] float8_e4m3fn or, two elements per byte, [rows, Kp / 2] uint8 (element 2i in the low nibble), Kp = K
+    rounded up to a multiple of 128; `scales` [ceil(rows / 128), Kp / 128, 32, 4, 4] float8_e8m0fnu, entry (R, T, i, j,
+    b) that of row 128 R + 32 j + i and block 4 T + b. What fills up K and the rows is zero codes and scale 2^-127."""
+
+    __slots__ = ("fmt", "shape", "dtype", "rows", "k", "buf", "codes_bytes", "__weakref__")
+
+    def __init__(self, shape, fmt, dtype, device):
+        if fmt not in MX_FORMATS:
+            raise ValueError(f"the format must be one of {sorted(MX_FORMATS)}, got {fmt!r}")
+        self.fmt, self.shape, self.dtype = fmt, torch.Size(shape), dtype
+        self.k = self.shape[-1]
+        self.rows = self.shape.numel() // self.k
+        kp = -(-self.k // 128) * 128
+        codes = self.rows * (kp // 2 if fmt == "mxfp4" else kp)
+        self.codes_bytes = -(-codes // 512) * 512  # the scales follow on a 512-byte boundary
+        scales = -(-self.rows // 128) * 4 * kp
+        self.buf = torch.empty(self.codes_bytes + scales, dtype=torch.uint8, device=device)
+
+    @property
+    def device(self):
+        return self.buf.device
+
+    def _ptrs(self):
+        p = self.buf.data_ptr()
+        return p, p + self.codes_bytes
+
+    @property
+    def codes(self):
+        kp = -(-self.k // 128) * 128
+        if self.fmt == "mxfp4":
+            return self.buf[:self.rows * kp // 2].view(self.rows, kp // 2)
+        return self.buf[:self.rows * kp].view(torch.float8_e4m3fn).view(self.rows, kp)
+
+    @property
+    def scales(self):
+        return self.buf[self.codes_bytes:].view(torch.float8_e8m0fnu).view(-(-self.rows // 128), -(-self.k // 128), 32, 4, 4)
+
+    def dequantize(self, dtype=torch.float32):
+        """The values that the codes and scales stand for, rounded once to `dtype`, in the logical shape."""
+        if dtype not in MX_DTYPES:
+            raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+        out = torch.empty(self.shape, dtype=dtype, device=self.buf.device)
+        c, s = self._ptrs()
+        _call_on(self.buf.device, "ko_dequantize_mx", c, s, MX_FORMATS[self.fmt], self.rows, self.k, out.data_ptr(),
+                 MX_DTYPES[dtype])
+        return out
+
+
+def quantize_mx(x, fmt="mxfp4") -> MXTensor:
+    """x [..., K] float32, bfloat16 or float16 (any even row pitch) in a microscaled format: per block of 32 along K the
+    scale 2^(floor(log2(max |x|)) - 2) (mxfp4; - 8 for mxfp8), held to 2^-127 or above, and x / scale to the nearest
+    element, ties to even, saturating. A block holding a NaN or an infinity becomes NaN."""
+    rows, pitch = _rows(x, "x")
+    q = MXTensor(x.shape, fmt, x.dtype, x.device)
+    c, s = q._ptrs()
+    _call_on(x.device, "ko_quantize_mx", x.data_ptr(), MX_DTYPES[x.dtype], rows, q.k, pitch, MX_FORMATS[fmt], c, s)
+    return q
+
+
+def residual_rmsnorm(h, o, bias, scale, gamma, eps, quantize=None, h_out=None):
+    """Returns (v, y) with v = h + (o + bias) * scale and y = v / sqrt(mean(v^2) + eps) * gamma over the last dimension
+    (width <= 32768), both computed in fp32: residual_layernorm's arguments for a model that normalises by the root
+    mean square. h and o: [..., C] float32, bfloat16 or float16 (any even row pitch); bias and scale [C] or None (0 / 1);
+    gamma [C]; all of one type. v is returned in that type, in h_out where given ([..., C] contiguous, possibly h); y
+    too, or with quantize "mxfp8" / "mxfp4" as an MXTensor, quantised from fp32 in the same pass."""
+    rows, ldh = _rows(h, "h")
+    if o.shape != h.shape:
+        raise ValueError("h and o must have the same shape")
+    _, ldo = _rows(o, "o", h.dtype, h.device)
+    if h_out is None:
+        h_out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    elif h_out.shape != h.shape or h_out.dtype != h.dtype or h_out.device != h.device or not h_out.is_contiguous():
+        raise ValueError("h_out must be contiguous, of h's shape, type and device")
+    return h_out, _rmsnorm(h, rows, ldh, o.data_ptr(), ldo, bias, scale, gamma, eps, quantize, h_out.data_ptr())
+
+
+def rmsnorm(x, gamma, eps, quantize=None):
+    """x / sqrt(mean(x^2) + eps) * gamma over the last dimension: residual_rmsnorm without a residual. Returns y."""
+    rows, ldx = _rows(x, "x")
+    return _rmsnorm(x, rows, ldx, None, 0, None, None, gamma, eps, quantize, None)
+
+
+def _rmsnorm(h, rows, ldh, o_ptr, ldo, bias, scale, gamma, eps, quantize, h_out_ptr):
+    c, dt, dev = h.shape[-1], h.dtype, h.device
+    if gamma is None:
+        raise ValueError("gamma is required")
+    params = (_vector(bias, "bias", c, dt, dev), _vector(scale, "scale", c, dt, dev),
+              _vector(gamma, "gamma", c, dt, dev))
+    if quantize is None:
+        y = torch.empty(h.shape, dtype=dt, device=dev)
+        to = (y.data_ptr(), 0, None, None)
+    else:
+        y = MXTensor(h.shape, quantize, dt, dev)
+        to = (None, MX_FORMATS[quantize], *y._ptrs())
+    _call_on(dev, "ko_residual_rmsnorm", h.data_ptr(), ldh, o_ptr, ldo, *params, MX_DTYPES[dt], float(eps), rows, c,
+             h_out_ptr, *to)
+    return y
+
+
+class PackedWeightMX:
+    """A [K, N] weight as its transpose in mxfp4 (blocks along K), with its bias in fp32: linear_mxfp4's operand."""
+
+    __slots__ = ("mx", "k", "n", "bias", "__weakref__")
+
+    def __init__(self, w, bias=None):
+        if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype not in MX_DTYPES:
+            raise ValueError("w must be a float32, bfloat16 or float16 CUDA tensor (there is no CPU path)")
+        if w.dim() != 2 or not w.is_contiguous() or w.numel() == 0:
+            raise ValueError("w must be [K, N], contiguous and not empty")
+        self.k, self.n = w.shape
+        if bias is not None and (not isinstance(bias, torch.Tensor) or bias.device != w.device
+                                 or bias.dtype not in MX_DTYPES or bias.numel() != self.n):
+            raise ValueError(f"bias must hold {self.n} float32, bfloat16 or float16 elements on {w.device}")
+        self.mx = MXTensor((self.n, self.k), "mxfp4", w.dtype, w.device)
+        c, s = self.mx._ptrs()
+        _call_on(w.device, "ko_pack_weight_mxfp4", w.data_ptr(), MX_DTYPES[w.dtype], self.k, self.n, c, s)
+        self.bias = None if bias is None else bias.detach().reshape(-1).to(torch.float32, copy=True)
+        status_word(w.device)
+
+    def dequantize(self, dtype=torch.float32):
+        """The [K, N] values that the packed weight stands for."""
+        return self.mx.dequantize(dtype).t()
+
+
+def pack_weight_mxfp4(w, bias=None) -> PackedWeightMX:
+    """Quantises w [K, N] (x @ W) once for linear_mxfp4. The bias is copied."""
+    return PackedWeightMX(w, bias)
+
+
+def linear_mxfp4(x, pw: PackedWeightMX, act=None, out_dtype=None, out=None):
+    """act(x @ W + bias) with W in mxfp4, on the block-scaled tensor-core products with fp32 accumulation. x: an
+    MXTensor [..., K] (mxfp8 or mxfp4), or a float32 / bfloat16 / float16 tensor, which is quantised to mxfp4 first. act
+    None, 'gelu' or 'relu'. The output [..., N] is rounded once, to out_dtype (x's type by default)."""
+    if act not in ACTS:
+        raise ValueError(f"act must be one of {list(ACTS)}")
+    if not isinstance(x, MXTensor):
+        if isinstance(x, torch.Tensor) and x.dim() and x.shape[-1] != pw.k:
+            raise ValueError(f"x has {x.shape[-1]} features, the weight expects {pw.k}")
+        x = quantize_mx(x, "mxfp4")
+    elif x.k != pw.k:
+        raise ValueError(f"x has {x.k} features, the weight expects {pw.k}")
+    dev = x.buf.device
+    if dev != pw.mx.buf.device:
+        raise ValueError(f"x is on {dev}, the weight on {pw.mx.buf.device}")
+    shape = (*x.shape[:-1], pw.n)
+    if out is None:
+        dt = x.dtype if out_dtype is None else out_dtype
+        if dt not in MX_DTYPES:
+            raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {dt}")
+        out = torch.empty(shape, dtype=dt, device=dev)
+    elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.device != dev
+          or not out.is_contiguous() or out.dtype not in MX_DTYPES or out_dtype not in (None, out.dtype)):
+        raise ValueError(f"out must be a contiguous {list(shape)} tensor on {dev}, float32, bfloat16 or float16")
+    _call_on(dev, "ko_linear_mxfp4", *x._ptrs(), MX_FORMATS[x.fmt], *pw.mx._ptrs(), _ptr(pw.bias), x.rows, pw.k, pw.n,
+             ACTS[act], out.data_ptr(), MX_DTYPES[out.dtype], status_word(dev).data_ptr())
     return out

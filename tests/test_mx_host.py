@@ -1,0 +1,126 @@
+"""The microscaled entry points refuse bad arguments on the host, before any device work, and the oracle of their
+formats holds against hand-computed values. No GPU needed."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import oracle.mx as OM
+from kernelopt_b200 import _lib
+from kernelopt_b200 import kernels as K
+
+A = 4096  # a stand-in for an aligned device pointer: every call below is refused before it is used
+
+
+@pytest.mark.parametrize("name,args", [
+    ("ko_quantize_mx", (A, 0, -1, 64, 64, 0, A, A, None)),                # rows < 0
+    ("ko_quantize_mx", (A, 0, 4, 0, 64, 0, A, A, None)),                  # K = 0
+    ("ko_quantize_mx", (A, 0, 4, 64, 63, 0, A, A, None)),                 # pitch below the width
+    ("ko_quantize_mx", (A, 3, 4, 64, 64, 0, A, A, None)),                 # unknown element type
+    ("ko_quantize_mx", (A, 0, 4, 64, 64, 2, A, A, None)),                 # unknown format
+    ("ko_quantize_mx", (A + 2, 0, 4, 64, 64, 0, A, A, None)),             # x not aligned to its elements
+    ("ko_quantize_mx", (A, 0, 4, 64, 64, 0, A + 8, A, None)),             # codes unaligned
+    ("ko_quantize_mx", (A, 0, 4, 64, 64, 0, A, None, None)),              # no scales
+    ("ko_quantize_mx", (A, 0, 1 << 31, 1 << 24, 1 << 24, 0, A, A, None)),  # more blocks than a grid holds
+    ("ko_dequantize_mx", (A, A, 0, 4, 0, A, 0, None)),                    # K = 0
+    ("ko_dequantize_mx", (A, A, 5, 4, 64, A, 0, None)),                   # unknown format
+    ("ko_dequantize_mx", (A, A, 0, 4, 64, None, 0, None)),                # no output
+    ("ko_dequantize_mx", (A, A + 4, 0, 4, 64, A, 0, None)),               # scales unaligned
+    ("ko_pack_weight_mxfp4", (A, 0, 0, 64, A, A, None)),                  # K = 0
+    ("ko_pack_weight_mxfp4", (A, 0, 64, 0, A, A, None)),                  # N = 0
+    ("ko_pack_weight_mxfp4", (A, 7, 64, 64, A, A, None)),                 # unknown element type
+    ("ko_pack_weight_mxfp4", (None, 0, 64, 64, A, A, None)),              # no weight
+    ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, A, 0, 1e-6, 4, 0, A, A, 0, None, None, None)),      # C = 0
+    ("ko_residual_rmsnorm", (A, 1 << 16, A, 1 << 16, None, None, A, 0, 1e-6, 4, 32769, A, A, 0, None, None, None)),
+    ("ko_residual_rmsnorm", (A, 63, A, 64, None, None, A, 0, 1e-6, 4, 64, A, A, 0, None, None, None)),     # ldh < C
+    ("ko_residual_rmsnorm", (A, 64, A, 63, None, None, A, 0, 1e-6, 4, 64, A, A, 0, None, None, None)),     # ldo < C
+    ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, A, 0, -1.0, 4, 64, A, A, 0, None, None, None)),     # eps < 0
+    ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, A, 0, float("nan"), 4, 64, A, A, 0, None, None, None)),
+    ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, None, 0, 1e-6, 4, 64, A, A, 0, None, None, None)),  # no gamma
+    ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, A, 0, 1e-6, 4, 64, A, A, 0, A, A, None)),           # y and codes
+    ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, A, 0, 1e-6, 4, 64, A, None, 0, A, None, None)),     # no scales
+    ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, A, 0, 1e-6, 4, 64, A, None, 9, A, A, None)),        # format
+    ("ko_residual_rmsnorm", (A, 64, None, 0, A, None, A, 0, 1e-6, 4, 64, A, A, 0, None, None, None)),      # bias, no o
+    ("ko_residual_rmsnorm", (A, 72, A, 64, None, None, A, 0, 1e-6, 4, 64, A, A, 0, None, None, None)),     # h_out is a
+    ("ko_residual_rmsnorm", (A, 64, A + 1, 64, None, None, A, 1, 1e-6, 4, 64, A, A, 0, None, None, None)),  # strided h
+    ("ko_linear_mxfp4", (A, A, 0, A, A, None, -1, 64, 64, 0, A, 0, None, None)),   # M < 0
+    ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 0, 64, 0, A, 0, None, None)),     # K = 0
+    ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 64, 0, 0, A, 0, None, None)),     # N = 0
+    ("ko_linear_mxfp4", (A, A, 2, A, A, None, 4, 64, 64, 0, A, 0, None, None)),    # unknown format
+    ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 64, 64, 3, A, 0, None, None)),    # SiLU not offered
+    ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 64, 64, 0, A, 4, None, None)),    # unknown output type
+    ("ko_linear_mxfp4", (A, A, 0, A, None, None, 4, 64, 64, 0, A, 0, None, None)),  # no weight scales
+    ("ko_linear_mxfp4", (A + 8, A, 0, A, A, None, 4, 64, 64, 0, A, 0, None, None)),  # codes unaligned
+    ("ko_linear_mxfp4", (A, A, 0, A, A, A + 2, 4, 64, 64, 0, A, 0, None, None)),   # bias unaligned
+    ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 64, 64, 0, A + 1, 1, None, None)),  # out unaligned
+])
+def test_bad_arguments_are_refused_on_the_host(name, args):
+    with pytest.raises(ValueError, match=name):
+        _lib.call(name, *args)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("ko_quantize_mx", (None, 0, 0, 64, 64, 0, None, None, None)),
+    ("ko_dequantize_mx", (None, None, 0, 0, 64, None, 0, None)),
+    ("ko_residual_rmsnorm", (None, 64, None, 0, None, None, None, 0, 1e-6, 0, 64, None, None, 0, None, None, None)),
+    ("ko_linear_mxfp4", (None, None, 0, None, None, None, 0, 64, 64, 0, None, 0, None, None)),
+])
+def test_no_rows_is_no_work(name, args):
+    assert _lib.call(name, *args) == _lib.KO_OK
+
+
+def test_sizes():
+    lib = _lib.lib()
+    assert lib.ko_mx_codes_bytes(3, 100, _lib.KO_MXFP4) == 3 * 64
+    assert lib.ko_mx_codes_bytes(3, 129, _lib.KO_MXFP8) == 3 * 256
+    assert lib.ko_mx_scales_bytes(129, 129) == 256 * 8
+    assert lib.ko_mx_codes_bytes(3, 0, 0) == lib.ko_mx_codes_bytes(-1, 8, 0) == lib.ko_mx_codes_bytes(3, 8, 2) == -1
+    assert lib.ko_mx_scales_bytes(-1, 8) == lib.ko_mx_scales_bytes(1, 0) == -1
+
+
+def test_python_entry_points_refuse_cpu_tensors_and_unknown_names():
+    x, w = torch.zeros(4, 64), torch.zeros(64, 8)
+    for call in (lambda: K.quantize_mx(x), lambda: K.residual_rmsnorm(x, x, None, None, x[0], 1e-6),
+                 lambda: K.rmsnorm(x, x[0], 1e-6), lambda: K.pack_weight_mxfp4(w)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+    with pytest.raises(ValueError, match="act"):
+        K.linear_mxfp4(x, None, act="silu")
+    with pytest.raises(ValueError, match="format"):
+        K.MXTensor((4, 64), "mxfp6", torch.float32, "cpu")
+
+
+def test_row_pitch_rules():
+    """The pitch of evenly spaced rows, and the refusals, on tensors without a device (the check for CUDA apart)."""
+    class Fake(torch.Tensor):
+        is_cuda = True
+
+    t = torch.zeros(6, 4, 40).as_subclass(Fake)
+    assert K._rows(t, "t") == (24, 40)
+    assert K._rows(t[..., 8:], "t") == (24, 40)
+    assert K._rows(t[:, :1, 3:7], "t") == (6, 160)
+    assert K._rows(t[0, 0, 3:7], "t") == (1, 4)
+    assert K._rows(t[:0], "t") == (0, 40)
+    assert K._rows(t[..., :1], "t") == (24, 40)
+    for bad in (t[:, :3], t.transpose(1, 2), t[..., ::2], t[:1, :1].expand(2, 3, 40), t[0, 0, 0], t[..., :0]):
+        with pytest.raises(ValueError):
+            K._rows(bad, "t")
+    with pytest.raises(ValueError):
+        K._rows(t.double(), "t")
+
+
+def test_oracle_against_hand_computed_blocks():
+    v = np.zeros((1, 64))
+    v[0, :8] = [6, 5, 2.5, 1.75, 0.25, 0.75, -3.5, 7.9]       # ties: 5 -> 4, 2.5 -> 2, 1.75 -> 2, 0.25 -> 0, 0.75 -> 1
+    v[0, 32:36] = [2.0 ** -140, -(2.0 ** -128), 0, 2.0 ** -129]
+    q = OM.round_trip(v, "mxfp4")
+    assert q[0, :8].tolist() == [6, 4, 2, 2, 0, 1, -4, 6]
+    assert q[0, 32:36].tolist() == [0, -(2.0 ** -128), 0, 0]
+    codes, scales = OM.quantize(v, "mxfp4")
+    assert scales.tolist() == [[127, 0, 0, 0]] and codes[0, 6] == 8 + 6
+    v[0, :4] = [500, 448, 1.0625, 2.0 ** -9]
+    q = OM.round_trip(v, "mxfp8")
+    assert q[0, :4].tolist() == [448, 448, 1.0, 2.0 ** -9]    # saturated; 1.0625 is a tie and goes to the even 1
+    v[0, 1] = np.inf
+    assert np.isnan(OM.round_trip(v, "mxfp8")[0, :32]).all() and np.isfinite(OM.round_trip(v, "mxfp8")[0, 32:]).all()
