@@ -338,10 +338,19 @@ int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, int64_t ldo, 
 
 /* out = act(A @ W^T + bias): A [M][K] in a_fmt (KO_MXFP4 or KO_MXFP8), W [N][K] in KO_MXFP4 (ko_pack_weight_mxfp4),
  * bias float32 [N] or NULL, fp32 accumulation, act KO_ACT_NONE, KO_ACT_GELU (erf form) or KO_ACT_RELU, out [M][N] of
- * `out_dtype`, contiguous. Codes and scales as above; dev_status as for ko_linear_f32_packed. */
+ * `out_dtype`, contiguous. Codes and scales as above, the weight's codes on 32 bytes; dev_status as for
+ * ko_linear_f32_packed. */
 int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_fmt, const void* w_codes, const void* w_scales,
                     const float* bias, int64_t M, int64_t K, int64_t N, int act, void* out, int out_dtype,
                     int* dev_status, ko_stream_t stream);
+
+/* The same for a few rows that are not quantised yet: x [M][K] of x_dtype, row r at x + r * ldx elements, is quantised to
+ * KO_MXFP4 inside the product's kernel, with the result of ko_quantize_mx and ko_linear_mxfp4 bit for bit. For the tokens
+ * of a decoding step, where a launch of its own and the round trip through memory cost more than the quantisation. */
+#define KO_MXFP4_FUSED_ROWS 16
+int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx, const void* w_codes, const void* w_scales,
+                             const float* bias, int64_t M, int64_t K, int64_t N, int act, void* out, int out_dtype,
+                             int* dev_status, ko_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,6 +21,7 @@ KO_RESIZE_REFERENCE, KO_RESIZE_OPENCV = 0, 1
 KO_ACT_NONE, KO_ACT_GELU, KO_ACT_RELU, KO_ACT_SILU = 0, 1, 2, 3
 KO_F32, KO_BF16, KO_F16 = 0, 1, 2
 KO_MXFP4, KO_MXFP8 = 0, 1
+KO_MXFP4_FUSED_ROWS = 16
 
 _i64, _i32, _f32, _vp = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
 
@@ -67,6 +68,7 @@ SIGNATURES = {
     "ko_pack_weight_mxfp4": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp]),
     "ko_residual_rmsnorm": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _f32, _i64, _i64, _vp, _vp, _i32, _vp,
                                    _vp, _vp]),
+    "ko_linear_quantize_mxfp4": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _vp]),
     "ko_linear_mxfp4": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _vp]),
 }
 
@@ -107,7 +109,7 @@ LAUNCHING = {"ko_preprocess": 1, "ko_preprocess_batch": 1, "ko_residual_layernor
              "ko_wait_probe": 1, "ko_window_merge_ln": 1, "ko_window_partition_ln": 1, "ko_deform_prep": 1,
              "ko_linear_add_f32_packed": 1, "ko_sine_embed": 1, "ko_linear_small_f32": 1, "ko_box_head_f32": 1,
              "ko_quantize_mx": 1, "ko_dequantize_mx": 1, "ko_pack_weight_mxfp4": 1, "ko_residual_rmsnorm": 1,
-             "ko_linear_mxfp4": 1}
+             "ko_linear_mxfp4": 1, "ko_linear_quantize_mxfp4": 1}
 launch_count: dict[str, int] = {}
 
 

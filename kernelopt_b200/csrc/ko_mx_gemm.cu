@@ -1,99 +1,859 @@
 // Product of microscaled operands:  out[M][N] = act(A[M][K] @ W[N][K]^T + bias),  A in mxfp4 or mxfp8, W in mxfp4.
 // Formats and layout: ko_mx.cuh.
 //
-// 64 x 64 tiles: 256 threads expand 32 elements along K of both operands to fp32 in shared memory and accumulate
-// 4 x 4 outputs each in fp32.
+// The 5th-generation tensor cores multiply the codes and apply both blocks' scales in the same instruction
+// (tcgen05.mma ... block_scale), accumulating in fp32 in tensor memory:
+//   A in mxfp4: kind::mxf4, 64 elements along K per instruction, both operands packed two per byte
+//   A in mxfp8: kind::mxf8f6f4, 32 elements along K per instruction; the 4-bit weight stays packed in HBM and TMA spreads
+//               it to one element per byte in shared memory, as that kind reads it
+// An operand row is 128 bytes of shared memory per pipeline stage (256 mxfp4 or 128 mxfp8 elements), 128-byte swizzled. The
+// scales of 128 rows x 128 elements are one 512-byte tile in HBM; TMA brings the stage's tiles in and tcgen05.cp spreads
+// them over tensor memory, ahead of the stage's MMAs on the same pipe.
+//
+// Two kernels: pairs of CTAs with 256 x 256 tiles for many rows (pair_kernel), and single CTAs over slices of K for few
+// (slice_kernel). Every wait is bounded; a wait that runs out ends the kernel with KO_ERR_DEVICE_TIMEOUT in *dev_status.
+#include <algorithm>
+#include <atomic>
+#include <climits>
 #include <string>
+#include <type_traits>
 
 #include "ko_mx.cuh"
 
 namespace {
 
+using namespace kodev;
 using namespace komx;
 
-constexpr int kTile = 64;
-constexpr int kThreads = 256;
+// ---- tcgen05 block-scaled forms (PTX ISA, tcgen05.mma / tcgen05.cp) ----------------------------------------
 
-__device__ __forceinline__ float act_f(float v, int act) {
-  // 1 + erf(v / sqrt 2) as erfc(-v / sqrt 2), which keeps its relative accuracy where v is far below zero
-  if (act == KO_ACT_GELU) return 0.5f * v * erfcf(v * -0.7071067811865476f);
+// Instruction descriptor of the block-scaled kinds: element types at bits 7 and 10 (e2m1 is 1 in kind::mxf4 and 5 in
+// kind::mxf8f6f4, e4m3 is 0), N / 8 at bit 17, e8m0 scales at bit 23, M / 128 at bit 27. The scale bytes that an
+// instruction uses within its 32-bit scale word start at byte `sf`, given for A at bit 29 and for B at bit 4.
+__host__ __device__ constexpr uint32_t idesc_bs(uint32_t a_type, uint32_t b_type, int m, int n) {
+  return (a_type << 7) | (b_type << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(m >> 7) << 27);
+}
+__host__ __device__ constexpr uint32_t idesc_sf(uint32_t sf) { return (sf << 29) | (sf << 4); }
+
+// One elected lane issues; GROUP: CTAs whose tensor cores run the instruction as one.
+template <int GROUP, bool F4>
+__device__ __forceinline__ void mma_bs_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+#define KO_MMA_BS(FORM)                                                                                        \
+  asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %6, 0;\n\telect.sync _|e, 0xffffffff;\n\t"             \
+               "@e tcgen05.mma." FORM " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),                       \
+               "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                 \
+               : "memory")
+  if constexpr (GROUP == 2 && F4) KO_MMA_BS("cta_group::2.kind::mxf4.block_scale.scale_vec::2X");
+  else if constexpr (GROUP == 2) KO_MMA_BS("cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X");
+  else if constexpr (F4) KO_MMA_BS("cta_group::1.kind::mxf4.block_scale.scale_vec::2X");
+  else KO_MMA_BS("cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X");
+#undef KO_MMA_BS
+}
+
+// 512 bytes of shared memory (32 rows of 16 bytes) to four tensor-memory columns, the same in all four lane quarters. With
+// GROUP 2 both CTAs of the pair copy, each from its own shared memory.
+template <int GROUP>
+__device__ __forceinline__ void cp_scales_w(uint32_t taddr, uint64_t desc) {
+  if constexpr (GROUP == 2)
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Shared-memory descriptor of a scale tile: no swizzle, 8-row groups of 16-byte rows 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 16) |
+         (static_cast<uint64_t>(128u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(ncols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Arrive on `bar` in both CTAs of the pair when every MMA issued so far has completed.
+__device__ __forceinline__ void mma_commit_pair_w(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b16 mask;\n\tmov.b16 mask, 3;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], mask;\n\t}" ::"r"(
+          smem_addr(bar))
+      : "memory");
+}
+// TMA load into this CTA's shared memory whose bytes count on a barrier of the pair's leader (`bar`: shared::cluster).
+__device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t bar, void* dst, int32_t c0, int32_t c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ float cluster_load_f(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool wait_cluster_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const bool ok = mbar_wait_cluster(bar, parity, abort);
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <bool F4>
+struct Elem {
+  static constexpr uint32_t kTypeA = F4 ? 1u : 0u;  // e2m1 / e4m3
+  static constexpr uint32_t kTypeW = F4 ? 1u : 5u;  // e2m1 in either kind's numbering
+  static constexpr int kStageK = F4 ? 256 : 128;    // elements along K per stage: 128 bytes of shared memory per row
+  static constexpr int kKt = kStageK / 128;         // scale tiles along K per stage
+  static constexpr int kMma = 4;                    // instructions along K per stage, 32 bytes each
+  // What a barrier counts for a box of 128 weight rows: the bytes that TMA reads. A spread box reads half of what it fills.
+  static constexpr uint32_t kTxW = 128 * (F4 ? 128 : 64);
+  // scale word (tile along K) and first scale byte of instruction j
+  static constexpr __host__ __device__ int kt_of(int j) { return F4 ? j >> 1 : 0; }
+  static constexpr __host__ __device__ uint32_t sf_of(int j) { return F4 ? static_cast<uint32_t>(j & 1) * 2 : j; }
+};
+
+__device__ __forceinline__ float apply_act(float v, int act) {
+  if (act == KO_ACT_GELU) return gelu_as7126(v);
   if (act == KO_ACT_RELU) return v < 0.f ? 0.f : v;
   return v;
 }
 
-template <int FMT>
-__device__ __forceinline__ void expand8(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                        int64_t row, int64_t rows, int64_t pitch, int64_t ktiles, int64_t k,
-                                        float (&v)[8]) {
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// pair_kernel: persistent CTA pairs (clusters of two), 256 x 256 output tiles. The pair's tensor cores run as one
+// (cta_group::2): each CTA holds 128 rows of A and 128 of the 256 weight rows of a stage and receives its 128 x 256 half
+// of the product in its own tensor memory, so an SM loads 32 KB of codes per stage for twice the work of a 128 x 128 tile.
+//   warp 0       TMA producer of this CTA; its bytes count on the leader's `full` barrier
+//   warp 1       tensor memory; in the leader it copies the scales and issues the MMAs of both CTAs
+//   warps 2-9    epilogue: two warps per lane quarter; accumulator -> + bias, activation, one rounding -> a swizzled
+//                tile in shared memory -> TMA store (rows of `out` on 16 bytes), or element stores (any other N)
+// Tensor memory (512 columns): two accumulators of 256 columns that share [128, 256), the scales in [384, 512) with a slot
+// per stage. The epilogue drains the shared half first and then lets the next tile's MMAs go, so all but the drain of
+// half a tile overlaps them.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int kPairThreads = 10 * 32;
+constexpr int kPairTile = 256;
+
+template <bool F4>
+struct PairCfg {
+  static constexpr int kStages = 5;
+  static constexpr uint32_t kOperand = 128 * 128;
+  static constexpr uint32_t kSfa = 512 * Elem<F4>::kKt, kSfb = 2 * kSfa;
+  static constexpr uint32_t kOffSf = 2 * kOperand;
+  static constexpr uint32_t kStage = (2 * kOperand + kSfa + kSfb + 1023) / 1024 * 1024;
+  static constexpr uint32_t kTx = 2 * (kOperand + Elem<F4>::kTxW + kSfa + kSfb);  // both CTAs
+  static constexpr uint32_t kOffStaging = kStages * kStage;
+  static constexpr uint32_t kStaging = 32 * 128;  // one warp's 32 rows of 128 bytes
+  static constexpr uint32_t kOffBars = kOffStaging + 8 * kStaging;
+  static constexpr uint32_t kSmem = 1024 + kOffBars + 256;
+  static constexpr uint32_t kColSf = 384, kSfCols = 12 * Elem<F4>::kKt;  // per slot: A 4, W 8 per scale tile along K
+  static_assert(kColSf + kStages * kSfCols <= 512, "tensor memory");
+  static_assert((2 * kStages + 3) * 8 + 16 <= 256, "barrier area");
+};
+
+struct PairArgs {
+  const float* bias;
+  void* out;
+  int* dev_status;
+  int64_t M, N;
+  int act, k_stages, m_tiles, n_tiles, n_pairs, tma_out;
+};
+
+template <bool F4, typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sw,
+                const __grid_constant__ CUtensorMap map_out, const PairArgs a) {
+  using C = PairCfg<F4>;
+  using E = Elem<F4>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);  // stage landed in both CTAs (leader: 1 + tx)
+  uint64_t* empty = full + C::kStages;    // stage's MMAs done            (1 commit, both CTAs)
+  uint64_t* acc_full = empty + C::kStages;  // tile's MMAs done           (1 commit, both CTAs)
+  uint64_t* acc_free = acc_full + 1;      // shared half drained          (8 warps x 2 CTAs, leader)
+  uint64_t* mma_done = acc_full + 2;      // every MMA done               (1 commit, both CTAs)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 3);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = static_cast<int>(blockIdx.x >> 1);
+  const int total = a.m_tiles * a.n_tiles;
+  // Tiles in bands of eight row tiles, rows fastest: the pairs that run together share few strips of A and W.
+  auto tile_at = [&](int t, int& m, int& n) {
+    const int band = t / (8 * a.n_tiles), in = t - band * 8 * a.n_tiles;
+    const int rows = min(8, a.m_tiles - band * 8);
+    n = in / rows;
+    m = band * 8 + (in - n * rows);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 16);
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_w);
+    prefetch_tmap(&map_sa);
+    prefetch_tmap(&map_sw);
+    prefetch_tmap(&map_out);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised before any arrival from the peer
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t leader_full = cluster_map(smem_addr(full), 0);
+      for (int t = pair; t < total && ok; t += a.n_pairs) {
+        int mt, nt;
+        tile_at(t, mt, nt);
+        for (int ks = 0; ks < a.k_stages; ++ks) {
+          if (!mbar_wait(&empty[st], phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* s = smem + st * C::kStage;
+          const uint32_t bar = leader_full + st * 8;
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], C::kTx);
+          const int half = static_cast<int>(rank) * 128;
+          tma_load_2d_pair(&map_a, bar, s, ks * 128, mt * 256 + half);
+          tma_load_2d_pair(&map_w, bar, s + C::kOperand, ks * 128, nt * 256 + half);
+          tma_load_2d_pair(&map_sa, bar, s + C::kOffSf, ks * 64 * E::kKt, mt * 2 + static_cast<int>(rank));
+          tma_load_2d_pair(&map_sw, bar, s + C::kOffSf + C::kSfa, ks * 64 * E::kKt, nt * 2);
+          if (++st == C::kStages) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {  // the loads in flight must land before the CTA leaves; they take microseconds
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 10000000ull) {}
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc = idesc_bs(E::kTypeA, E::kTypeW, 256, 256);
+      const uint32_t sb = smem_addr(smem);
+      int st = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += a.n_pairs, ++local) {
+        if (local > 0 && !wait_cluster_warp(acc_free, static_cast<uint32_t>(local - 1) & 1u, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (local & 1) * 128;
+        for (int ks = 0; ks < a.k_stages; ++ks) {
+          if (!wait_cluster_warp(&full[st], phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t s = sb + st * C::kStage;
+          const uint32_t sfa = tmem + C::kColSf + st * C::kSfCols, sfb = sfa + 4 * E::kKt;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (row >= rows) return;
-  const float s = scale_value(scales[scale_word_offset(row, k >> 7, ktiles) + ((k >> 5) & 3)]);
-  if constexpr (FMT == KO_MXFP4) {
-    unpack_e2m1x8(*reinterpret_cast<const uint32_t*>(codes + row * pitch + k / 2), v);
+          for (int kt = 0; kt < E::kKt; ++kt) {
+            cp_scales_w<2>(sfa + 4 * kt, scale_desc(s + C::kOffSf + kt * 512));
+            cp_scales_w<2>(sfb + 8 * kt, scale_desc(s + C::kOffSf + C::kSfa + kt * 512));
+            cp_scales_w<2>(sfb + 8 * kt + 4, scale_desc(s + C::kOffSf + C::kSfa + (E::kKt + kt) * 512));
+          }
+#pragma unroll
+          for (int j = 0; j < E::kMma; ++j)
+            mma_bs_w<2, F4>(d, smem_desc_k_sw128(s + j * 32), smem_desc_k_sw128(s + C::kOperand + j * 32),
+                            idesc | idesc_sf(E::sf_of(j)), sfa + 4 * E::kt_of(j), sfb + 8 * E::kt_of(j),
+                            (ks > 0 || j > 0) ? 1u : 0u);
+          mma_commit_pair_w(&empty[st]);
+          if (++st == C::kStages) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) mma_commit_pair_w(acc_full);
+      }
+      mma_commit_pair_w(mma_done);
+    }
+    volatile int never = 0;
+    if (!mbar_wait_warp(mma_done, 0, &never)) *abort_flag = 1;
   } else {
+    const int q = warp & 3, h = (warp - 2) >> 2;
+    uint8_t* staging = smem + C::kOffStaging + (warp - 2) * C::kStaging;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const uint32_t free_bar = cluster_map(smem_addr(acc_free), 0);
+    constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a staging row
+    int local = 0;
+    for (int t = pair; t < total; t += a.n_pairs, ++local) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      if (!mbar_wait_warp(acc_full, static_cast<uint32_t>(local) & 1u, abort_flag)) break;
+      tc_fence_after();
+      const int64_t row0 = static_cast<int64_t>(mt) * 256 + rank * 128 + q * 32;
+#pragma unroll 1
+      for (int g = 0; g < 2; ++g) {
+        const int col = (g == 0 ? 128 : (local & 1) ? 256 : 0) + h * 64;  // tensor-memory column
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(lane_base + col, r[0]);
+        tmem_ld_32x32b_x32(lane_base + col + 32, r[1]);
+        tmem_ld_wait_regs(r[0]);
+        tmem_ld_wait_regs(r[1]);
+        if (g == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(free_bar);
+        }
+        const int64_t col0 = static_cast<int64_t>(nt) * 256 + col - (local & 1) * 128;
+        if (row0 >= a.M || col0 >= a.N) continue;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack_e4m3x2(*reinterpret_cast<const uint16_t*>(codes + row * pitch + k + 2 * i));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int64_t n = col0 + c * 32 + j;
+            const float b = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
+            r[c][j] = __float_as_uint(apply_act(__uint_as_float(r[c][j]) + b, a.act));
+          }
+#pragma unroll
+        for (int part = 0; part < 64 / kCols; ++part) {  // one staging tile: 64 columns of 16 bits or 32 of 32
+          if (a.tma_out) {
+            if (lane == 0) bulk_wait_read<0>();
+          }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint4 v;
+            if constexpr (sizeof(T) == 2) {
+              const uint32_t* p = &r[j >> 2][(j & 3) * 8];
+              v = make_uint4(pack2<T>(__uint_as_float(p[0]), __uint_as_float(p[1])),
+                             pack2<T>(__uint_as_float(p[2]), __uint_as_float(p[3])),
+                             pack2<T>(__uint_as_float(p[4]), __uint_as_float(p[5])),
+                             pack2<T>(__uint_as_float(p[6]), __uint_as_float(p[7])));
+            } else {
+              v = make_uint4(r[part][j * 4], r[part][j * 4 + 1], r[part][j * 4 + 2], r[part][j * 4 + 3]);
+            }
+            *reinterpret_cast<uint4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+          }
+          const int64_t pc = col0 + part * kCols;
+          if (a.tma_out) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && pc < a.N) {
+              tma_store_2d(&map_out, staging, static_cast<int32_t>(pc), static_cast<int32_t>(row0));
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            T* out = static_cast<T*>(a.out);
+            const int rows = static_cast<int>(min(int64_t(32), a.M - row0));
+            for (int rr = 0; rr < rows; ++rr)
+              for (int c = lane; c < kCols; c += 32)
+                if (pc + c < a.N) {
+                  const int byte = c * static_cast<int>(sizeof(T));
+                  out[(row0 + rr) * a.N + pc + c] = *reinterpret_cast<const T*>(
+                      staging + rr * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
+                }
+          }
+        }
+      }
     }
+    if (lane == 0) bulk_wait<0>();  // the stores have left shared memory and are written
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= s;
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other's arrivals, copies or MMAs may still reach it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag && a.dev_status) atomicExch(a.dev_status, KO_ERR_DEVICE_TIMEOUT);
 }
 
-template <int FMT, typename T>
-__global__ void __launch_bounds__(kThreads)
-    linear_kernel(const uint8_t* __restrict__ ac, const uint8_t* __restrict__ as, const uint8_t* __restrict__ wc,
-                  const uint8_t* __restrict__ ws, const float* __restrict__ bias, int64_t M, int64_t N, int64_t Kp,
-                  int act, T* __restrict__ out, int64_t n_tiles) {
-  __shared__ float sa[32][kTile + 1], sw[32][kTile + 1];
-  const int64_t m0 = blockIdx.x / n_tiles * kTile, n0 = blockIdx.x % n_tiles * kTile;
-  const int lr = threadIdx.x >> 2, lk = (threadIdx.x & 3) * 8;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t a_pitch = FMT == KO_MXFP4 ? Kp / 2 : Kp;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < Kp; k0 += 32) {
-    float v[8];
-    expand8<FMT>(ac, as, m0 + lr, M, a_pitch, Kp / 128, k0 + lk, v);
+// ---------------------------------------------------------------------------------------------------------
+// slice_kernel: few rows of A. The weight's rows take the MMA's 128-row side and A's rows (BN of them) its narrow side, so
+// the product comes out transposed: a thread owns one output column and a warp writes 32 neighbours of a row at a time, for
+// any N. The CTAs of a cluster share a tile and take a slice of K each; their partial sums meet in shared memory and are
+// added in rank order through distributed shared memory, so results repeat bit for bit.
+// With XT other than void the rows of A come as XT values, at most kFuseRows of them, and warps 2 and 3 quantise them to
+// mxfp4 on the way into shared memory, a block of 32 to a thread: for a handful of tokens that costs less than a launch of
+// its own, and every CTA needs only its slice of them.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int kSliceThreads = 128;
+constexpr int kFuseRows = KO_MXFP4_FUSED_ROWS;
+
+template <bool F4, int BN>
+struct SliceCfg {
+  static constexpr uint32_t kW = 128 * 128, kX = BN * 128, kSf = 512 * Elem<F4>::kKt;
+  static constexpr uint32_t kOffSf = kW + kX;
+  static constexpr uint32_t kStage = (kW + kX + 2 * kSf + 1023) / 1024 * 1024;
+  static constexpr uint32_t kTx = Elem<F4>::kTxW + kX + 2 * kSf;
+  static constexpr int kStages = BN <= 32 ? 5 : BN <= 64 ? 4 : 3;  // about 100 KB: two CTAs share an SM
+  static constexpr uint32_t kOffBars = kStages * kStage;
+  static constexpr uint32_t kSmem = 1024 + kOffBars + 256;
+  static constexpr uint32_t kAccCols = BN < 32 ? 32 : BN;
+  static constexpr uint32_t kSfCols = 8 * Elem<F4>::kKt;
+  static constexpr uint32_t kNeed = kAccCols + kStages * kSfCols;
+  static constexpr uint32_t kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
+  static_assert(kNeed <= 256, "two CTAs of an SM share 512 columns");
+  static_assert(BN * 128 * 4 <= kOffBars, "partial sums reuse the stages");
+  static_assert((2 * kStages + 1) * 8 + 16 <= 256, "barrier area");
+};
+
+struct SliceArgs {
+  const float* bias;
+  void* out;
+  int* dev_status;
+  int64_t M, N;
+  int act, k_stages, n_tiles, slices;
+  const void* x;  // unquantised rows [M][K], ldx elements apart (XT other than void)
+  int64_t K, ldx;
+  int x_vec;      // rows of x start on 16 bytes
+};
+
+// A block of 32 elements from k on, zero beyond K: its mxfp4 codes and its scale byte.
+template <typename XT>
+__device__ __forceinline__ uint4 quantize_block(const XT* row, int64_t k, int64_t K, bool vec, uint32_t& byte) {
+  float v[4][8];
+  uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sa[lk + i][lr] = v[i];
-    expand8<KO_MXFP4>(wc, ws, n0 + lr, N, Kp / 2, Kp / 128, k0 + lk, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sw[lk + i][lr] = v[i];
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty + 16 * i], sw[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+  for (int g = 0; g < 4; ++g) {
+    if (vec) load8<XT, true>(row, k + g * 8, K, v[g]);
+    else load8<XT, false>(row, k + g * 8, K, v[g]);
+    m = max(m, amax_bits8(v[g]));
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < M && n < N) out[m * N + n] = from_f<T>(act_f(acc[i][j] + (bias ? bias[n] : 0.f), act));
-    }
+  byte = scale_byte<KO_MXFP4>(m);
+  if (byte == 255u) return make_uint4(0u, 0u, 0u, 0u);
+  const float inv = scale_inverse(byte);
+  return make_uint4(pack_e2m1x8(v[0], inv), pack_e2m1x8(v[1], inv), pack_e2m1x8(v[2], inv), pack_e2m1x8(v[3], inv));
 }
 
-template <int FMT>
-int launch(const uint8_t* ac, const uint8_t* as, const uint8_t* wc, const uint8_t* ws, const float* bias, int64_t M,
-           int64_t K, int64_t N, int act, void* out, int dtype, cudaStream_t s) {
-  const int64_t n_tiles = (N + kTile - 1) / kTile, blocks = (M + kTile - 1) / kTile * n_tiles, Kp = padded_k(K);
-  if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_linear_mxfp4: the output is too large");
-  const unsigned g = static_cast<unsigned>(blocks);
-  if (dtype == KO_F32)
-    linear_kernel<FMT><<<g, kThreads, 0, s>>>(ac, as, wc, ws, bias, M, N, Kp, act, static_cast<float*>(out), n_tiles);
-  else if (dtype == KO_BF16)
-    linear_kernel<FMT><<<g, kThreads, 0, s>>>(ac, as, wc, ws, bias, M, N, Kp, act, static_cast<__nv_bfloat16*>(out),
-                                              n_tiles);
-  else
-    linear_kernel<FMT><<<g, kThreads, 0, s>>>(ac, as, wc, ws, bias, M, N, Kp, act, static_cast<__half*>(out), n_tiles);
-  return ko::check_launch("ko_linear_mxfp4");
+template <bool F4, int BN, typename T, typename XT>
+__global__ void __launch_bounds__(kSliceThreads)
+    slice_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                 const __grid_constant__ CUtensorMap map_sx, const __grid_constant__ CUtensorMap map_sw,
+                 const SliceArgs a) {
+  using C = SliceCfg<F4, BN>;
+  using E = Elem<F4>;
+  constexpr bool kFuse = !std::is_void<XT>::value;
+  static_assert(!kFuse || (F4 && BN == kFuseRows), "fused quantisation is for mxfp4 and one tile of rows");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* acc_full = empty + C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = a.slices;
+  const int rank = static_cast<int>(blockIdx.x % S), tile = static_cast<int>(blockIdx.x / S);
+  const int nt = tile % a.n_tiles, mt = tile / a.n_tiles;
+  const int k0 = static_cast<int>(static_cast<int64_t>(a.k_stages) * rank / S);
+  const int k1 = static_cast<int>(static_cast<int64_t>(a.k_stages) * (rank + 1) / S);
+  const int64_t m0 = static_cast<int64_t>(mt) * BN;
+  const int cols = static_cast<int>(min(int64_t(BN), a.M - m0));  // rows of A in this tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], kFuse ? 3 : 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&map_w);
+    prefetch_tmap(&map_sw);
+    if (!kFuse) {
+      prefetch_tmap(&map_x);
+      prefetch_tmap(&map_sx);
+    }
+  }
+  if (kFuse && warp >= 2) {  // the scale tiles of x hold kFuseRows rows; the others are zero for good
+    for (int i = threadIdx.x - 64; i < C::kStages * static_cast<int>(C::kSf / 4); i += 64) {
+      const int st = i / static_cast<int>(C::kSf / 4), w = i % static_cast<int>(C::kSf / 4);
+      reinterpret_cast<uint32_t*>(smem + st * C::kStage + C::kOffSf + C::kSf)[w] = 0u;
+    }
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int ks = k0; ks < k1; ++ks) {
+        if (!mbar_wait(&empty[st], phase ^ 1u, abort_flag)) break;
+        uint8_t* s = smem + st * C::kStage;
+        mbar_arrive_expect_tx(&full[st], kFuse ? Elem<F4>::kTxW + C::kSf : C::kTx);
+        tma_load_2d(&map_w, &full[st], s, ks * 128, nt * 128);
+        tma_load_2d(&map_sw, &full[st], s + C::kOffSf, ks * 64 * E::kKt, nt);
+        if (!kFuse) {
+          tma_load_2d(&map_x, &full[st], s + C::kW, ks * 128, static_cast<int32_t>(m0));
+          tma_load_2d(&map_sx, &full[st], s + C::kOffSf + C::kSf, ks * 64 * E::kKt, static_cast<int32_t>(m0 / 128));
+        }
+        ++issued;
+        if (++st == C::kStages) {
+          st = 0;
+          phase ^= 1u;
+        }
+      }
+      // every load has landed before the CTA leaves: the last use of each stage, the only one that may be in flight
+      volatile int never = 0;
+      for (int s = 0; s < C::kStages && s < issued; ++s) {
+        const int last = (issued - 1 - s) / C::kStages;
+        if (!mbar_wait(&full[s], static_cast<uint32_t>(last) & 1u, &never)) *abort_flag = 1;
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = idesc_bs(E::kTypeW, E::kTypeA, 128, BN);
+    const uint32_t sb = smem_addr(smem);
+    int st = 0;
+    uint32_t phase = 0;
+    for (int ks = k0; ks < k1; ++ks) {
+      if (!mbar_wait_warp(&full[st], phase, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t s = sb + st * C::kStage;
+      const uint32_t sfw = tmem + C::kAccCols + st * C::kSfCols, sfx = sfw + 4 * E::kKt;
+#pragma unroll
+      for (int kt = 0; kt < E::kKt; ++kt) {
+        cp_scales_w<1>(sfw + 4 * kt, scale_desc(s + C::kOffSf + kt * 512));
+        cp_scales_w<1>(sfx + 4 * kt, scale_desc(s + C::kOffSf + C::kSf + kt * 512));
+      }
+#pragma unroll
+      for (int j = 0; j < E::kMma; ++j)
+        mma_bs_w<1, F4>(tmem, smem_desc_k_sw128(s + j * 32), smem_desc_k_sw128(s + C::kW + j * 32),
+                        idesc | idesc_sf(E::sf_of(j)), sfw + 4 * E::kt_of(j), sfx + 4 * E::kt_of(j),
+                        (ks > k0 || j > 0) ? 1u : 0u);
+      mma_commit_w(&empty[st]);
+      if (++st == C::kStages) {
+        st = 0;
+        phase ^= 1u;
+      }
+    }
+    mma_commit_w(acc_full);
+  } else if constexpr (kFuse) {
+    // Two blocks of the stage per thread: block b of rows r and r + 8. A block's codes are one 16-byte chunk of the row.
+    const int b = threadIdx.x & 7, r = (threadIdx.x - 64) >> 3;
+    int st = 0;
+    uint32_t phase = 0;
+    for (int ks = k0; ks < k1; ++ks) {
+      uint4 code[2];
+      uint32_t byte[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        code[i] = make_uint4(0u, 0u, 0u, 0u);
+        byte[i] = 0u;
+        const int64_t k = static_cast<int64_t>(ks) * E::kStageK + b * 32;
+        if (r + 8 * i < cols && k < a.K)
+          code[i] = quantize_block(static_cast<const XT*>(a.x) + (r + 8 * i) * a.ldx, k, a.K, a.x_vec != 0, byte[i]);
+      }
+      if (!mbar_wait_warp(&empty[st], phase ^ 1u, abort_flag)) break;
+      uint8_t* s = smem + st * C::kStage;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = r + 8 * i;
+        *reinterpret_cast<uint4*>(s + C::kW + row * 128 + ((b ^ (row & 7)) << 4)) = code[i];
+        s[C::kOffSf + C::kSf + (b >> 2) * 512 + row * 16 + (b & 3)] = static_cast<uint8_t>(byte[i]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st]);
+      if (++st == C::kStages) {
+        st = 0;
+        phase ^= 1u;
+      }
+    }
+  }
+  __syncwarp();
+  volatile int never = 0;  // also after an abort: what was issued completes before its memory is given back
+  if (!mbar_wait_warp(acc_full, 0, &never)) *abort_flag = 1;
+  tc_fence_after();
+
+  const int64_t n = static_cast<int64_t>(nt) * 128 + threadIdx.x;
+  const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
+  T* out = static_cast<T*>(a.out) + m0 * a.N + n;
+  float* part = reinterpret_cast<float*>(smem);  // [BN][128]: every load has been read by its MMAs
+  const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+#pragma unroll
+  for (int c = 0; c < (BN + 31) / 32; ++c) {
+    if (c * 32 >= cols) break;
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(lane_base + c * 32, r);
+    tmem_ld_wait_regs(r);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c * 32 + j < cols) {
+        const float v = __uint_as_float(r[j]);
+        if (S > 1) part[(c * 32 + j) * 128 + threadIdx.x] = v;
+        else if (n < a.N) out[(c * 32 + j) * a.N] = from_f<T>(apply_act(v + bias, a.act));
+      }
+  }
+  tc_fence_before();
+  if (S > 1) {
+    cluster_sync();
+    const uint32_t mine = smem_addr(part) + threadIdx.x * 4;
+    for (int j = rank; j < cols; j += S) {
+      float v = 0.f;
+      for (int s = 0; s < S; ++s) v += cluster_load_f(cluster_map(mine + j * 512, static_cast<uint32_t>(s)));
+      if (n < a.N) out[j * a.N] = from_f<T>(apply_act(v + bias, a.act));
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+  if (threadIdx.x == 0 && *abort_flag && a.dev_status) atomicExch(a.dev_status, KO_ERR_DEVICE_TIMEOUT);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------
+
+int encode_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t cols, uint64_t rows,
+              uint64_t pitch_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle, const char* what) {
+  ko::EncodeTiledFn enc = ko::encode_tiled();
+  if (!enc) return ko::fail(KO_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch_bytes};
+  cuuint32_t box[2] = {box_cols, box_rows}, estr[2] = {1, 1};
+  const CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return ko::fail(KO_ERR_INVALID_ARGUMENT,
+                    std::string(what) + ": cuTensorMapEncodeTiled failed (CUresult " + std::to_string(r) + ")");
+  return KO_OK;
+}
+// Boxes of 128 shared-memory bytes x box_rows rows; `spread`: 4-bit codes to one per byte.
+int encode_codes(CUtensorMap* map, const void* codes, int fmt, bool spread, int64_t rows, int64_t Kp, uint32_t box_rows,
+                 const char* what) {
+  const uint64_t pitch = static_cast<uint64_t>(fmt == KO_MXFP4 ? Kp / 2 : Kp);
+  if (spread)
+    return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, codes, Kp, rows, pitch, 128, box_rows,
+                     CU_TENSOR_MAP_SWIZZLE_128B, what);
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, pitch, rows, pitch, 128, box_rows,
+                   CU_TENSOR_MAP_SWIZZLE_128B, what);
+}
+// Scale tiles as rows of 64 8-byte words per tile; boxes of kt tiles along K x row_tiles.
+int encode_scales(CUtensorMap* map, const void* scales, int64_t rows, int64_t Kp, int kt, uint32_t row_tiles,
+                  const char* what) {
+  const uint64_t words = static_cast<uint64_t>(Kp / 128) * 64;
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, scales, words, static_cast<uint64_t>((rows + 127) / 128),
+                   words * 8, 64u * kt, row_tiles, CU_TENSOR_MAP_SWIZZLE_NONE, what);
+}
+
+struct Call {
+  const void *ac, *as, *wc, *ws;
+  const float* bias;
+  int64_t M, K, N, Kp;
+  int act;
+  void* out;
+  int* dev_status;
+  cudaStream_t stream;
+  const ko::DeviceInfo* info;
+  const void* x;  // unquantised A (fused form)
+  int64_t ldx;
+};
+
+// The opt-in to more than 48 KB of shared memory, once per kernel and device.
+template <typename Kernel>
+int allow_smem(Kernel kernel, std::atomic<bool>* done, int dev, uint32_t bytes) {
+  if (done[dev].load(std::memory_order_relaxed)) return KO_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e != cudaSuccess) return ko::fail(static_cast<int>(e), "ko_linear_mxfp4: shared memory");
+  done[dev].store(true, std::memory_order_relaxed);
+  return KO_OK;
+}
+constexpr int kMaxDevices = 64;
+int current_device() {  // device_or_fail has accepted it, so it is below kMaxDevices
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+
+cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* attr, unsigned cluster, unsigned blocks, unsigned threads,
+                                  size_t smem, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+template <bool F4, typename T>
+int launch_pair(const Call& c) {
+  using C = PairCfg<F4>;
+  using E = Elem<F4>;
+  constexpr const char* who = "ko_linear_mxfp4";
+  const int64_t mt = (c.M + kPairTile - 1) / kPairTile, nt = (c.N + kPairTile - 1) / kPairTile;
+  if (mt * nt > INT32_MAX / 16) return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(who) + ": too many output tiles");
+  CUtensorMap ma, mw, msa, msw, mo;
+  const int64_t es = static_cast<int64_t>(sizeof(T));
+  const bool tma_out = ko::aligned16(c.out) && c.N * es % 16 == 0;
+  int rc = encode_codes(&ma, c.ac, F4 ? KO_MXFP4 : KO_MXFP8, false, c.M, c.Kp, 128, who);
+  if (!rc) rc = encode_codes(&mw, c.wc, KO_MXFP4, !F4, c.N, c.Kp, 128, who);
+  if (!rc) rc = encode_scales(&msa, c.as, c.M, c.Kp, E::kKt, 1, who);
+  if (!rc) rc = encode_scales(&msw, c.ws, c.N, c.Kp, E::kKt, 2, who);
+  mo = ma;  // not used without tma_out
+  if (!rc && tma_out)
+    rc = encode_2d(&mo, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, c.out, c.N, c.M,
+                   c.N * es, static_cast<uint32_t>(128 / es), 32, CU_TENSOR_MAP_SWIZZLE_128B, who);
+  if (rc) return rc;
+  PairArgs a{};
+  a.bias = c.bias;
+  a.out = c.out;
+  a.dev_status = c.dev_status;
+  a.M = c.M;
+  a.N = c.N;
+  a.act = c.act;
+  a.k_stages = static_cast<int>((c.Kp + E::kStageK - 1) / E::kStageK);
+  a.m_tiles = static_cast<int>(mt);
+  a.n_tiles = static_cast<int>(nt);
+  a.tma_out = tma_out ? 1 : 0;
+  auto kernel = pair_kernel<F4, T>;
+  static std::atomic<bool> allowed[kMaxDevices];
+  static std::atomic<int> resident[kMaxDevices];  // CTA pairs that the device holds at once, found once per device
+  const int dev = current_device();
+  rc = allow_smem(kernel, allowed, dev, C::kSmem);
+  if (rc) return rc;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg =
+      cluster_config(attr, 2, 2 * static_cast<unsigned>(c.info->sm_count / 2), kPairThreads, C::kSmem, c.stream);
+  int pairs = resident[dev].load(std::memory_order_relaxed);
+  if (pairs <= 0) {
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg);
+    if (e != cudaSuccess) return ko::fail(static_cast<int>(e), std::string(who) + ": occupancy");
+    pairs = std::max(pairs, 1);
+    resident[dev].store(pairs, std::memory_order_relaxed);
+  }
+  a.n_pairs = static_cast<int>(std::min<int64_t>(mt * nt, pairs));
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(a.n_pairs));
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ma, mw, msa, msw, mo, a);
+  if (e != cudaSuccess) return ko::fail(static_cast<int>(e), std::string(who) + ": launch failed");
+  return ko::check_launch(who);
+}
+
+template <bool F4, int BN, typename T, typename XT = void>
+int launch_slice(const Call& c) {
+  constexpr bool kFuse = !std::is_void<XT>::value;
+  using C = SliceCfg<F4, BN>;
+  using E = Elem<F4>;
+  constexpr const char* who = "ko_linear_mxfp4";
+  const int64_t mt = (c.M + BN - 1) / BN, nt = (c.N + 127) / 128;
+  if (mt * nt > INT32_MAX / 16) return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(who) + ": too many output tiles");
+  CUtensorMap mx, mw, msx, msw;
+  int rc = encode_codes(&mw, c.wc, KO_MXFP4, !F4, c.N, c.Kp, 128, who);
+  if (!rc) rc = encode_scales(&msw, c.ws, c.N, c.Kp, E::kKt, 1, who);
+  if (kFuse) {
+    mx = mw;  // not used
+    msx = msw;
+  } else {
+    if (!rc) rc = encode_codes(&mx, c.ac, F4 ? KO_MXFP4 : KO_MXFP8, false, c.M, c.Kp, BN, who);
+    if (!rc) rc = encode_scales(&msx, c.as, c.M, c.Kp, E::kKt, 1, who);
+  }
+  if (rc) return rc;
+  SliceArgs a{};
+  if constexpr (kFuse) {
+    a.x = c.x;
+    a.K = c.K;
+    a.ldx = c.ldx;
+    a.x_vec = ko::aligned16(c.x) && c.ldx * static_cast<int64_t>(sizeof(XT)) % 16 == 0;
+  }
+  a.bias = c.bias;
+  a.out = c.out;
+  a.dev_status = c.dev_status;
+  a.M = c.M;
+  a.N = c.N;
+  a.act = c.act;
+  a.k_stages = static_cast<int>((c.Kp + E::kStageK - 1) / E::kStageK);
+  a.n_tiles = static_cast<int>(nt);
+  int slices = 1;
+  while (slices < 8 && mt * nt * slices * 2 <= 2 * c.info->sm_count && slices * 2 <= a.k_stages) slices *= 2;
+  a.slices = slices;
+  auto kernel = slice_kernel<F4, BN, T, XT>;
+  static std::atomic<bool> allowed[kMaxDevices];
+  rc = allow_smem(kernel, allowed, current_device(), C::kSmem);
+  if (rc) return rc;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = cluster_config(attr, slices, static_cast<unsigned>(mt * nt * slices), kSliceThreads, C::kSmem,
+                                          c.stream);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, msx, msw, a);
+  if (e != cudaSuccess) return ko::fail(static_cast<int>(e), std::string(who) + ": launch failed");
+  return ko::check_launch(who);
+}
+
+template <bool F4, typename T>
+int launch(const Call& c) {
+  const int64_t pair_tiles = ((c.M + 255) / 256) * ((c.N + 255) / 256);
+  if (c.M > 128 && pair_tiles >= 24) return launch_pair<F4, T>(c);
+  if (c.M <= 16) return launch_slice<F4, 16, T>(c);
+  if (c.M <= 32) return launch_slice<F4, 32, T>(c);
+  if (c.M <= 64) return launch_slice<F4, 64, T>(c);
+  return launch_slice<F4, 128, T>(c);
+}
+
+template <typename T>
+int launch_fused(const Call& c, int x_dtype) {
+  if (x_dtype == KO_F32) return launch_slice<true, kFuseRows, T, float>(c);
+  if (x_dtype == KO_BF16) return launch_slice<true, kFuseRows, T, __nv_bfloat16>(c);
+  return launch_slice<true, kFuseRows, T, __half>(c);
+}
+
+int check_linear(const char* name, int64_t M, int64_t K, int64_t N, int act, const void* w_codes, const void* w_scales,
+                 const float* bias, const void* out, int out_dtype) {
+  auto bad = [&](const char* what) { return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
+  if (M < 0 || M > kMaxRows || K < 1 || K > kMaxK || N < 1 || N > kMaxRows)
+    return bad("need 0 <= M <= 2^31, 1 <= K <= 2^24 and 1 <= N <= 2^31");
+  if (!dtype_ok(out_dtype)) return bad("unknown output type");
+  if (act != KO_ACT_NONE && act != KO_ACT_GELU && act != KO_ACT_RELU)
+    return bad("act must be KO_ACT_NONE, KO_ACT_GELU or KO_ACT_RELU");
+  if (M == 0) return KO_OK;
+  if (!w_codes || !w_scales || !out) return bad("null pointer");
+  if (reinterpret_cast<uintptr_t>(w_codes) % 32 != 0 || !ko::aligned16(w_scales))
+    return bad("the weight's codes must be 32-byte aligned, its scales 16");
+  if (reinterpret_cast<uintptr_t>(out) % static_cast<uintptr_t>(dtype_size(out_dtype)) != 0 ||
+      reinterpret_cast<uintptr_t>(bias) % 4 != 0)
+    return bad("out and bias must be aligned to their elements");
+  return KO_OK;
 }
 
 }  // namespace
@@ -101,25 +861,41 @@ int launch(const uint8_t* ac, const uint8_t* as, const uint8_t* wc, const uint8_
 extern "C" int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_fmt, const void* w_codes,
                                const void* w_scales, const float* bias, int64_t M, int64_t K, int64_t N, int act,
                                void* out, int out_dtype, int* dev_status, ko_stream_t stream) {
-  const std::string who = "ko_linear_mxfp4: ";
-  if (M < 0 || M > kMaxRows || K < 1 || K > kMaxK || N < 1 || N > kMaxRows)
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "need 0 <= M <= 2^31, 1 <= K <= 2^24 and 1 <= N <= 2^31");
-  if (!fmt_ok(a_fmt) || !dtype_ok(out_dtype))
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "unknown format or output type");
-  if (act != KO_ACT_NONE && act != KO_ACT_GELU && act != KO_ACT_RELU)
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "act must be KO_ACT_NONE, KO_ACT_GELU or KO_ACT_RELU");
+  const char* name = "ko_linear_mxfp4";
+  int rc = check_linear(name, M, K, N, act, w_codes, w_scales, bias, out, out_dtype);
+  if (rc) return rc;
+  if (!fmt_ok(a_fmt)) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_linear_mxfp4: unknown format");
   if (M == 0) return KO_OK;
-  if (!a_codes || !a_scales || !w_codes || !w_scales || !out)
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
-  if (!ko::aligned16(a_codes) || !ko::aligned16(a_scales) || !ko::aligned16(w_codes) || !ko::aligned16(w_scales))
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "codes and scales must be 16-byte aligned");
-  if (reinterpret_cast<uintptr_t>(out) % static_cast<uintptr_t>(dtype_size(out_dtype)) != 0 ||
-      reinterpret_cast<uintptr_t>(bias) % 4 != 0)
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "out and bias must be aligned to their elements");
-  const uint8_t *ac = static_cast<const uint8_t*>(a_codes), *as = static_cast<const uint8_t*>(a_scales);
-  const uint8_t *wc = static_cast<const uint8_t*>(w_codes), *ws = static_cast<const uint8_t*>(w_scales);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  (void)dev_status;
-  return a_fmt == KO_MXFP4 ? launch<KO_MXFP4>(ac, as, wc, ws, bias, M, K, N, act, out, out_dtype, s)
-                           : launch<KO_MXFP8>(ac, as, wc, ws, bias, M, K, N, act, out, out_dtype, s);
+  if (!a_codes || !a_scales || !ko::aligned16(a_codes) || !ko::aligned16(a_scales))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_linear_mxfp4: codes and scales must be given, 16-byte aligned");
+  Call c{a_codes, a_scales, w_codes, w_scales, bias, M, K, N, padded_k(K), act, out, dev_status,
+         reinterpret_cast<cudaStream_t>(stream), nullptr, nullptr, 0};
+  rc = ko::device_or_fail(&c.info, name);
+  if (rc) return rc;
+  const bool f4 = a_fmt == KO_MXFP4;
+  if (out_dtype == KO_F32) return f4 ? launch<true, float>(c) : launch<false, float>(c);
+  if (out_dtype == KO_BF16) return f4 ? launch<true, __nv_bfloat16>(c) : launch<false, __nv_bfloat16>(c);
+  return f4 ? launch<true, __half>(c) : launch<false, __half>(c);
+}
+
+extern "C" int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx, const void* w_codes,
+                                        const void* w_scales, const float* bias, int64_t M, int64_t K, int64_t N,
+                                        int act, void* out, int out_dtype, int* dev_status, ko_stream_t stream) {
+  const char* name = "ko_linear_quantize_mxfp4";
+  int rc = check_linear(name, M, K, N, act, w_codes, w_scales, bias, out, out_dtype);
+  if (rc) return rc;
+  auto bad = [&](const char* what) { return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
+  if (!dtype_ok(x_dtype)) return bad("unknown element type");
+  if (M > kFuseRows) return bad("at most KO_MXFP4_FUSED_ROWS rows; more are quantised by ko_quantize_mx first");
+  if (ldx < K) return bad("ldx must be at least K");
+  if (M == 0) return KO_OK;
+  if (!x || reinterpret_cast<uintptr_t>(x) % static_cast<uintptr_t>(dtype_size(x_dtype)) != 0)
+    return bad("x must be given, aligned to its elements");
+  Call c{nullptr, nullptr, w_codes, w_scales, bias, M, K, N, padded_k(K), act, out, dev_status,
+         reinterpret_cast<cudaStream_t>(stream), nullptr, x, ldx};
+  rc = ko::device_or_fail(&c.info, name);
+  if (rc) return rc;
+  if (out_dtype == KO_F32) return launch_fused<float>(c, x_dtype);
+  if (out_dtype == KO_BF16) return launch_fused<__nv_bfloat16>(c, x_dtype);
+  return launch_fused<__half>(c, x_dtype);
 }

@@ -542,12 +542,18 @@ MX_FORMATS = {"mxfp4": _lib.KO_MXFP4, "mxfp8": _lib.KO_MXFP8}
 MX_DTYPES = {torch.float32: _lib.KO_F32, torch.bfloat16: _lib.KO_BF16, torch.float16: _lib.KO_F16}
 
 
+# The current stream's handle without building a Stream object (3 us a call, as much as a launch), where torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call_on(device, name, *args):
     """call(name, *args, stream) on the current stream of `device`, which need not be the current device."""
-    if device.index == torch.cuda.current_device():
-        return call(name, *args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        return call(name, *args, _raw_stream(index))
     with torch.cuda.device(device):
-        return call(name, *args, torch.cuda.current_stream().cuda_stream)
+        return call(name, *args, _raw_stream(index))
 
 
 def _rows(t, name, dtype=None, device=None):
@@ -603,38 +609,39 @@ class MXTensor:
     rounded up to a multiple of 128; `scales` [ceil(rows / 128), Kp / 128, 32, 4, 4] float8_e8m0fnu, entry (R, T, i, j,
     b) that of row 128 R + 32 j + i and block 4 T + b. What fills up K and the rows is zero codes and scale 2^-127."""
 
-    __slots__ = ("fmt", "shape", "dtype", "rows", "k", "buf", "codes_bytes", "__weakref__")
+    __slots__ = ("fmt", "shape", "dtype", "rows", "k", "buf", "__weakref__")
 
     def __init__(self, shape, fmt, dtype, device):
         if fmt not in MX_FORMATS:
             raise ValueError(f"the format must be one of {sorted(MX_FORMATS)}, got {fmt!r}")
         self.fmt, self.shape, self.dtype = fmt, torch.Size(shape), dtype
-        self.k = self.shape[-1]
-        self.rows = self.shape.numel() // self.k
-        kp = -(-self.k // 128) * 128
-        codes = self.rows * (kp // 2 if fmt == "mxfp4" else kp)
-        self.codes_bytes = -(-codes // 512) * 512  # the scales follow on a 512-byte boundary
-        scales = -(-self.rows // 128) * 4 * kp
-        self.buf = torch.empty(self.codes_bytes + scales, dtype=torch.uint8, device=device)
+        self.k = k = self.shape[-1]
+        self.rows = rows = self.shape.numel() // k
+        # One buffer whose rows are rows of codes. The scales follow: a byte for 32 elements and every row of the tiles
+        # of 128 is, in rows of codes, a 32nd (mxfp8) or a 16th (mxfp4) of the tiles' rows.
+        kp, tile_rows = -(-k // 128) * 128, -(-rows // 128) * 128
+        if fmt == "mxfp4":
+            self.buf = torch.empty((rows + tile_rows // 16, kp // 2), dtype=torch.uint8, device=device)
+        else:
+            self.buf = torch.empty((rows + tile_rows // 32, kp), dtype=torch.float8_e4m3fn, device=device)
 
     @property
     def device(self):
         return self.buf.device
 
     def _ptrs(self):
-        p = self.buf.data_ptr()
-        return p, p + self.codes_bytes
+        p, kp = self.buf.data_ptr(), -(-self.k // 128) * 128
+        return p, p + self.rows * (kp // 2 if self.fmt == "mxfp4" else kp)
 
     @property
     def codes(self):
-        kp = -(-self.k // 128) * 128
-        if self.fmt == "mxfp4":
-            return self.buf[:self.rows * kp // 2].view(self.rows, kp // 2)
-        return self.buf[:self.rows * kp].view(torch.float8_e4m3fn).view(self.rows, kp)
+        return self.buf[:self.rows]
 
     @property
     def scales(self):
-        return self.buf[self.codes_bytes:].view(torch.float8_e8m0fnu).view(-(-self.rows // 128), -(-self.k // 128), 32, 4, 4)
+        tiles, kt = -(-self.rows // 128), -(-self.k // 128)
+        return self.buf.view(torch.float8_e8m0fnu).as_strided(
+            (tiles, kt, 32, 4, 4), (kt * 512, 512, 16, 4, 1), self.rows * self.buf.shape[1])
 
     def dequantize(self, dtype=torch.float32):
         """The values that the codes and scales stand for, rounded once to `dtype`, in the logical shape."""
@@ -701,7 +708,7 @@ def _rmsnorm(h, rows, ldh, o_ptr, ldo, bias, scale, gamma, eps, quantize, h_out_
 class PackedWeightMX:
     """A [K, N] weight as its transpose in mxfp4 (blocks along K), with its bias in fp32: linear_mxfp4's operand."""
 
-    __slots__ = ("mx", "k", "n", "bias", "__weakref__")
+    __slots__ = ("mx", "k", "n", "bias", "ptrs", "status", "__weakref__")
 
     def __init__(self, w, bias=None):
         if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype not in MX_DTYPES:
@@ -716,7 +723,9 @@ class PackedWeightMX:
         c, s = self.mx._ptrs()
         _call_on(w.device, "ko_pack_weight_mxfp4", w.data_ptr(), MX_DTYPES[w.dtype], self.k, self.n, c, s)
         self.bias = None if bias is None else bias.detach().reshape(-1).to(torch.float32, copy=True)
-        status_word(w.device)
+        # what every product with this weight passes: its addresses, and the device's status word, which never moves
+        self.ptrs = (c, s, _ptr(self.bias))
+        self.status = status_word(w.device).data_ptr()
 
     def dequantize(self, dtype=torch.float32):
         """The [K, N] values that the packed weight stands for."""
@@ -730,19 +739,21 @@ def pack_weight_mxfp4(w, bias=None) -> PackedWeightMX:
 
 def linear_mxfp4(x, pw: PackedWeightMX, act=None, out_dtype=None, out=None):
     """act(x @ W + bias) with W in mxfp4, on the block-scaled tensor-core products with fp32 accumulation. x: an
-    MXTensor [..., K] (mxfp8 or mxfp4), or a float32 / bfloat16 / float16 tensor, which is quantised to mxfp4 first. act
-    None, 'gelu' or 'relu'. The output [..., N] is rounded once, to out_dtype (x's type by default)."""
+    MXTensor [..., K] (mxfp8 or mxfp4), or a float32 / bfloat16 / float16 tensor, which is quantised to mxfp4 (up to 16
+    rows inside the product's kernel, more in a pass before it). act None, 'gelu' or 'relu'. The output [..., N] is rounded once, to out_dtype (x's type by default)."""
     if act not in ACTS:
         raise ValueError(f"act must be one of {list(ACTS)}")
-    if not isinstance(x, MXTensor):
-        if isinstance(x, torch.Tensor) and x.dim() and x.shape[-1] != pw.k:
-            raise ValueError(f"x has {x.shape[-1]} features, the weight expects {pw.k}")
-        x = quantize_mx(x, "mxfp4")
-    elif x.k != pw.k:
-        raise ValueError(f"x has {x.k} features, the weight expects {pw.k}")
-    dev = x.buf.device
-    if dev != pw.mx.buf.device:
-        raise ValueError(f"x is on {dev}, the weight on {pw.mx.buf.device}")
+    wdev = pw.mx.buf.device
+    quantized = isinstance(x, MXTensor)
+    if quantized:
+        rows, dev = x.rows, x.buf.device
+    else:
+        rows, pitch = _rows(x, "x")
+        dev = x.device
+    if x.shape[-1] != pw.k:
+        raise ValueError(f"x has {x.shape[-1]} features, the weight expects {pw.k}")
+    if dev != wdev:
+        raise ValueError(f"x is on {dev}, the weight on {wdev}")
     shape = (*x.shape[:-1], pw.n)
     if out is None:
         dt = x.dtype if out_dtype is None else out_dtype
@@ -752,6 +763,10 @@ def linear_mxfp4(x, pw: PackedWeightMX, act=None, out_dtype=None, out=None):
     elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.device != dev
           or not out.is_contiguous() or out.dtype not in MX_DTYPES or out_dtype not in (None, out.dtype)):
         raise ValueError(f"out must be a contiguous {list(shape)} tensor on {dev}, float32, bfloat16 or float16")
-    _call_on(dev, "ko_linear_mxfp4", *x._ptrs(), MX_FORMATS[x.fmt], *pw.mx._ptrs(), _ptr(pw.bias), x.rows, pw.k, pw.n,
-             ACTS[act], out.data_ptr(), MX_DTYPES[out.dtype], status_word(dev).data_ptr())
+    tail = (*pw.ptrs, rows, pw.k, pw.n, ACTS[act], out.data_ptr(), MX_DTYPES[out.dtype], pw.status)
+    if not quantized and rows <= _lib.KO_MXFP4_FUSED_ROWS:
+        _call_on(dev, "ko_linear_quantize_mxfp4", x.data_ptr(), MX_DTYPES[x.dtype], pitch, *tail)
+    else:
+        q = x if quantized else quantize_mx(x)
+        _call_on(dev, "ko_linear_mxfp4", *q._ptrs(), MX_FORMATS[q.fmt], *tail)
     return out

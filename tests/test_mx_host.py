@@ -54,6 +54,13 @@ A = 4096  # a stand-in for an aligned device pointer: every call below is refuse
     ("ko_linear_mxfp4", (A + 8, A, 0, A, A, None, 4, 64, 64, 0, A, 0, None, None)),  # codes unaligned
     ("ko_linear_mxfp4", (A, A, 0, A, A, A + 2, 4, 64, 64, 0, A, 0, None, None)),   # bias unaligned
     ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 64, 64, 0, A + 1, 1, None, None)),  # out unaligned
+    ("ko_linear_mxfp4", (A, A, 0, A + 16, A, None, 4, 64, 64, 0, A, 0, None, None)),  # weight codes not on 32 bytes
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 17, 64, 64, 0, A, 0, None, None)),   # too many rows
+    ("ko_linear_quantize_mxfp4", (A, 0, 63, A, A, None, 4, 64, 64, 0, A, 0, None, None)),    # pitch below the width
+    ("ko_linear_quantize_mxfp4", (A, 5, 64, A, A, None, 4, 64, 64, 0, A, 0, None, None)),    # unknown element type
+    ("ko_linear_quantize_mxfp4", (None, 0, 64, A, A, None, 4, 64, 64, 0, A, 0, None, None)),  # no x
+    ("ko_linear_quantize_mxfp4", (A + 1, 1, 64, A, A, None, 4, 64, 64, 0, A, 0, None, None)),  # x unaligned
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 4, 64, 64, 9, A, 0, None, None)),    # unknown act
 ])
 def test_bad_arguments_are_refused_on_the_host(name, args):
     with pytest.raises(ValueError, match=name):
