@@ -270,24 +270,6 @@ __device__ __forceinline__ uint32_t f32_to_tf32_rna(float x) {
 // f32_to_tf32_rna for every finite input, infinities included; NaNs stay NaNs.
 __device__ __forceinline__ uint32_t f32_to_tf32_rna_int(float x) { return (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u; }
 
-// GELU(v) = v * Phi(v), Phi the standard normal CDF = (1 + erf(v / sqrt 2)) / 2, with erfc(x) for x >= 0 from
-// Abramowitz & Stegun, Handbook of Mathematical Functions, formula 7.1.26: erfc(x) = t (a1 + t (a2 + ... + t a5))
-// exp(-x^2), t = 1 / (1 + p x), absolute error below 1.5e-7. With x = |v| / sqrt 2 and q = erfc(x) / 2 (the
-// factors 1/sqrt 2 and 1/2 folded into p and the a_i): Phi(v) = 1 - q for v >= 0 and q for v < 0.
-__device__ __forceinline__ float gelu_as7126(float v) {
-  const float ax = fabsf(v);
-  const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.7071067811865476f, ax, 1.0f));
-  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f),
-                                               0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f);
-  float e;  // exp(-v^2 / 2) as 2^(-v^2 log2(e) / 2)
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * v * -0.7213475204444817f));
-  const float q = poly * e;
-  const float vq = v * q;
-  // q underflows to 0 for large |v|: GELU(v) = v there (+inf included, where v * q would be inf * 0), and
-  // v * q keeps -inf -> NaN, as 0.5 * v * (1 + erf(v / sqrt 2)) gives
-  return v >= 0.0f ? (q > 0.0f ? v - vq : v) : vq;
-}
-
 // ---- thread-block clusters (distributed shared memory between the CTAs of one cluster) ----
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

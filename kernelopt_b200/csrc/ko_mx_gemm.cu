@@ -119,10 +119,61 @@ struct Elem {
   static constexpr __host__ __device__ uint32_t sf_of(int j) { return F4 ? static_cast<uint32_t>(j & 1) * 2 : j; }
 };
 
-__device__ __forceinline__ float apply_act(float v, int act) {
-  if (act == KO_ACT_GELU) return gelu_as7126(v);
-  if (act == KO_ACT_RELU) return v < 0.f ? 0.f : v;
-  return v;
+// ---- activation ----
+// Two fp32 values in one 64-bit register: Blackwell's packed multiply and fused multiply-add.
+__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// GELU of two values: v Phi(v) = max(v, 0) - |v| q with q = erfc(|v| / sqrt 2) / 2 = exp(-v^2 / 2) g(|v|). g is smooth
+// on [0, 6] (it falls from 1/2 to 0.066), so a polynomial of degree 12 in |v| / 3 - 1 has it, fitted by least squares at
+// Chebyshev nodes: q is within 3e-5 of itself everywhere, so the far negative side keeps its small values, and |v| q
+// within 8e-8. Beyond 6, g stays at its last value; q is below 1e-9 there. NaN stays NaN, and GELU(-inf) is 0, its limit.
+// Without a division, it costs one special-function instruction; A&S 7.1.26 (two of them, no packed form) took 30 us more
+// of the 25664 x 1536 fp32 outputs of the backbone's fc1.
+__device__ __forceinline__ void gelu_pair(float& a, float& b) {
+  constexpr float g[13] = {-0.12151393294334412f, 0.10320935398340225f, -0.08236773312091827f, 0.062280356884002686f,
+                           -0.04567015543580055f, 0.03141380101442337f, -0.01772490330040455f, 0.013943932950496674f,
+                           -0.015077504329383373f, 0.0027330496814101934f, 0.004123609978705645f, 0.004027877002954483f,
+                           -0.004158561583608389f};
+  const uint64_t ax = pack_f2(fminf(fabsf(a), 6.f), fminf(fabsf(b), 6.f));
+  const uint64_t s = fma_f2(ax, pack_f2(1.f / 3.f, 1.f / 3.f), pack_f2(-1.f, -1.f));
+  uint64_t p = pack_f2(g[12], g[12]);
+#pragma unroll
+  for (int i = 11; i >= 0; --i) p = fma_f2(p, s, pack_f2(g[i], g[i]));
+  const uint64_t v = pack_f2(a, b);
+  float wa, wb, ma, mb;  // exp(-v^2 / 2) as 2^(-v^2 log2(e) / 2)
+  unpack_f2(mul_f2(mul_f2(v, v), pack_f2(-0.7213475204444817f, -0.7213475204444817f)), wa, wb);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(wa) : "f"(wa));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(wb) : "f"(wb));
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(ma) : "f"(a));
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(mb) : "f"(b));
+  unpack_f2(fma_f2(ax, mul_f2(p, pack_f2(wa, wb)), pack_f2(ma, mb)), a, b);
+}
+template <int N>
+__device__ __forceinline__ void apply_act(float (&v)[N], int act) {
+  if (act == KO_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) gelu_pair(v[i], v[i + 1]);
+  } else if (act == KO_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays
+  }
 }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -141,30 +192,31 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
 // of the product in its own tensor memory, so an SM loads 32 KB of codes per stage for twice the work of a 128 x 128 tile.
 //   warp 0       TMA producer of this CTA; its bytes count on the leader's `full` barrier
 //   warp 1       tensor memory; in the leader it copies the scales and issues the MMAs of both CTAs
-//   warps 2-9    epilogue: two warps per lane quarter; accumulator -> + bias, activation, one rounding -> a swizzled
-//                tile in shared memory -> TMA store (rows of `out` on 16 bytes), or element stores (any other N)
+//   warps 2-17   epilogue: per lane quarter four warps of 64 columns each; accumulator -> + bias, activation, one rounding
+//                -> a swizzled tile in shared memory -> TMA store (rows of `out` on 16 bytes), or element stores (other N)
 // Tensor memory (512 columns): two accumulators of 256 columns that share [128, 256), the scales in [384, 512) with a slot
-// per stage. The epilogue drains the shared half first and then lets the next tile's MMAs go, so all but the drain of
-// half a tile overlaps them.
+// per stage. Warps 2-9 read the shared half into registers and then let the next tile's MMAs go; warps 10-17 have until
+// the tile after it for the other half. So all but the read of half an accumulator overlaps the MMAs.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kPairThreads = 10 * 32;
+constexpr int kPairThreads = 18 * 32;
 constexpr int kPairTile = 256;
 
 template <bool F4>
 struct PairCfg {
-  static constexpr int kStages = 5;
+  static constexpr int kStages = 4;
   static constexpr uint32_t kOperand = 128 * 128;
   static constexpr uint32_t kSfa = 512 * Elem<F4>::kKt, kSfb = 2 * kSfa;
   static constexpr uint32_t kOffSf = 2 * kOperand;
   static constexpr uint32_t kStage = (2 * kOperand + kSfa + kSfb + 1023) / 1024 * 1024;
   static constexpr uint32_t kTx = 2 * (kOperand + Elem<F4>::kTxW + kSfa + kSfb);  // both CTAs
   static constexpr uint32_t kOffStaging = kStages * kStage;
-  static constexpr uint32_t kStaging = 32 * 128;  // one warp's 32 rows of 128 bytes
-  static constexpr uint32_t kOffBars = kOffStaging + 8 * kStaging;
+  static constexpr uint32_t kStaging = 32 * 128;  // 32 rows of 128 bytes for each epilogue warp
+  static constexpr uint32_t kOffBias = kOffStaging + 16 * kStaging;  // 64 columns for each epilogue warp
+  static constexpr uint32_t kOffBars = kOffBias + 16 * 64 * 4;
   static constexpr uint32_t kSmem = 1024 + kOffBars + 256;
   static constexpr uint32_t kColSf = 384, kSfCols = 12 * Elem<F4>::kKt;  // per slot: A 4, W 8 per scale tile along K
   static_assert(kColSf + kStages * kSfCols <= 512, "tensor memory");
-  static_assert((2 * kStages + 3) * 8 + 16 <= 256, "barrier area");
+  static_assert((2 * kStages + 6) * 8 + 16 <= 256, "barrier area");
 };
 
 struct PairArgs {
@@ -186,10 +238,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);  // stage landed in both CTAs (leader: 1 + tx)
   uint64_t* empty = full + C::kStages;    // stage's MMAs done            (1 commit, both CTAs)
-  uint64_t* acc_full = empty + C::kStages;  // tile's MMAs done           (1 commit, both CTAs)
-  uint64_t* acc_free = acc_full + 1;      // shared half drained          (8 warps x 2 CTAs, leader)
-  uint64_t* mma_done = acc_full + 2;      // every MMA done               (1 commit, both CTAs)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 3);
+  // A barrier's parity cannot tell a phase from the one after the next, so where a waiter may be two tiles behind the last
+  // arrival there is a barrier for even tiles and one for odd.
+  uint64_t* acc_full = empty + C::kStages;  // tile's MMAs done           (1 commit, both CTAs) x 2
+  uint64_t* own_free = acc_full + 2;      // unshared half read           (8 warps x 2 CTAs, leader) x 2
+  uint64_t* shared_free = acc_full + 4;   // shared half read             (8 warps x 2 CTAs, leader)
+  uint64_t* mma_done = acc_full + 5;      // every MMA done               (1 commit, both CTAs)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 6);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -209,8 +264,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_free, 16);
+    mbar_init(&acc_full[0], 1);
+    mbar_init(&acc_full[1], 1);
+    mbar_init(&own_free[0], 16);
+    mbar_init(&own_free[1], 16);
+    mbar_init(shared_free, 16);
     mbar_init(mma_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -271,7 +329,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; t < total && ok; t += a.n_pairs, ++local) {
-        if (local > 0 && !wait_cluster_warp(acc_free, static_cast<uint32_t>(local - 1) & 1u, abort_flag)) break;
+        // the previous tile's shared half, and the other half of the tile before it
+        if (local > 0 && !wait_cluster_warp(shared_free, static_cast<uint32_t>(local - 1) & 1u, abort_flag)) break;
+        if (local > 1 && !wait_cluster_warp(&own_free[local & 1], static_cast<uint32_t>((local >> 1) - 1) & 1u, abort_flag))
+          break;
         tc_fence_after();
         const uint32_t d = tmem + (local & 1) * 128;
         for (int ks = 0; ks < a.k_stages; ++ks) {
@@ -299,88 +360,108 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             phase ^= 1u;
           }
         }
-        if (ok) mma_commit_pair_w(acc_full);
+        if (ok) mma_commit_pair_w(&acc_full[local & 1]);
       }
       mma_commit_pair_w(mma_done);
     }
     volatile int never = 0;
     if (!mbar_wait_warp(mma_done, 0, &never)) *abort_flag = 1;
   } else {
-    const int q = warp & 3, h = (warp - 2) >> 2;
-    uint8_t* staging = smem + C::kOffStaging + (warp - 2) * C::kStaging;
+    const int e = warp - 2, q = warp & 3;
+    const bool shared_half = e < 8;
+    const int h = (e >> 2) & 1;  // which 64 columns of the half
+    uint8_t* stg = smem + C::kOffStaging + e * C::kStaging;
+    float* bias = reinterpret_cast<float*>(smem + C::kOffBias) + e * 64;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
-    const uint32_t free_bar = cluster_map(smem_addr(acc_free), 0);
+    const uint32_t free_bar = cluster_map(smem_addr(shared_half ? shared_free : own_free), 0);
     constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a staging row
-    int local = 0;
-    for (int t = pair; t < total; t += a.n_pairs, ++local) {
+    // first tensor-memory column and first column of the output of this warp's part of tile t (the local-th)
+    auto part_of = [&](int t, int local, int& col, int& row0, int& col0) {
       int mt, nt;
       tile_at(t, mt, nt);
-      if (!mbar_wait_warp(acc_full, static_cast<uint32_t>(local) & 1u, abort_flag)) break;
+      col = (shared_half ? 128 : (local & 1) ? 256 : 0) + h * 64;
+      row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32;
+      col0 = nt * 256 + col - (local & 1) * 128;
+    };
+    auto load_bias = [&](int col0, float& b0, float& b1) {  // columns 2 lane and 2 lane + 1
+      const int n = col0 + 2 * lane;
+      b0 = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
+      b1 = a.bias && n + 1 < a.N ? __ldg(a.bias + n + 1) : 0.f;
+    };
+    int local = 0, col, row0, col0;
+    part_of(pair, 0, col, row0, col0);
+    float b0, b1;
+    load_bias(col0, b0, b1);
+    for (int t = pair; t < total; t += a.n_pairs, ++local) {
+      __syncwarp();
+      *reinterpret_cast<float2*>(bias + 2 * lane) = make_float2(b0, b1);
+      __syncwarp();
+      const int tcol = col, r0 = row0, c0 = col0;
+      if (t + a.n_pairs < total) {  // the next tile's bias comes while this tile is worked on
+        part_of(t + a.n_pairs, local + 1, col, row0, col0);
+        load_bias(col0, b0, b1);
+      }
+      if (!mbar_wait_warp(&acc_full[local & 1], static_cast<uint32_t>(local >> 1) & 1u, abort_flag)) break;
       tc_fence_after();
-      const int64_t row0 = static_cast<int64_t>(mt) * 256 + rank * 128 + q * 32;
-#pragma unroll 1
-      for (int g = 0; g < 2; ++g) {
-        const int col = (g == 0 ? 128 : (local & 1) ? 256 : 0) + h * 64;  // tensor-memory column
-        uint32_t r[2][32];
-        tmem_ld_32x32b_x32(lane_base + col, r[0]);
-        tmem_ld_32x32b_x32(lane_base + col + 32, r[1]);
-        tmem_ld_wait_regs(r[0]);
-        tmem_ld_wait_regs(r[1]);
-        if (g == 0) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(free_bar);
+      uint32_t r[2][32];
+      tmem_ld_32x32b_x32(lane_base + tcol, r[0]);
+      tmem_ld_32x32b_x32(lane_base + tcol + 32, r[1]);
+      tmem_ld_wait_regs(r[0]);
+      tmem_ld_wait_regs(r[1]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(free_bar + (shared_half ? 0 : (local & 1) * 8));
+      if (r0 >= a.M || c0 >= a.N) continue;
+      constexpr bool kWide = sizeof(T) == 4;  // 32 columns fill a staging row, else all 64 do
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 b = reinterpret_cast<const float4*>(bias)[c * 8 + j];
+          v[4 * j] = __uint_as_float(r[c][4 * j]) + b.x;
+          v[4 * j + 1] = __uint_as_float(r[c][4 * j + 1]) + b.y;
+          v[4 * j + 2] = __uint_as_float(r[c][4 * j + 2]) + b.z;
+          v[4 * j + 3] = __uint_as_float(r[c][4 * j + 3]) + b.w;
         }
-        const int64_t col0 = static_cast<int64_t>(nt) * 256 + col - (local & 1) * 128;
-        if (row0 >= a.M || col0 >= a.N) continue;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int64_t n = col0 + c * 32 + j;
-            const float b = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
-            r[c][j] = __float_as_uint(apply_act(__uint_as_float(r[c][j]) + b, a.act));
-          }
-#pragma unroll
-        for (int part = 0; part < 64 / kCols; ++part) {  // one staging tile: 64 columns of 16 bits or 32 of 32
-          if (a.tma_out) {
-            if (lane == 0) bulk_wait_read<0>();
-          }
+        apply_act(v, a.act);
+        if (kWide || c == 0) {
+          if (lane == 0) bulk_wait_read<0>();  // the last store has left the tile
           __syncwarp();
+        }
+        if constexpr (kWide) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint4 v;
-            if constexpr (sizeof(T) == 2) {
-              const uint32_t* p = &r[j >> 2][(j & 3) * 8];
-              v = make_uint4(pack2<T>(__uint_as_float(p[0]), __uint_as_float(p[1])),
-                             pack2<T>(__uint_as_float(p[2]), __uint_as_float(p[3])),
-                             pack2<T>(__uint_as_float(p[4]), __uint_as_float(p[5])),
-                             pack2<T>(__uint_as_float(p[6]), __uint_as_float(p[7])));
-            } else {
-              v = make_uint4(r[part][j * 4], r[part][j * 4 + 1], r[part][j * 4 + 2], r[part][j * 4 + 3]);
-            }
-            *reinterpret_cast<uint4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(stg + lane * 128 + (((c * 4 + j) ^ (lane & 7)) << 4)) =
+                make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
+                           pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7]));
+          if (c == 0) continue;
+        }
+        const int pc = c0 + (kWide ? c * 32 : 0);
+        if (a.tma_out) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && pc < a.N) {
+            tma_store_2d(&map_out, stg, pc, r0);
+            bulk_commit();
           }
-          const int64_t pc = col0 + part * kCols;
-          if (a.tma_out) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0 && pc < a.N) {
-              tma_store_2d(&map_out, staging, static_cast<int32_t>(pc), static_cast<int32_t>(row0));
-              bulk_commit();
-            }
-          } else {
-            __syncwarp();
-            T* out = static_cast<T*>(a.out);
-            const int rows = static_cast<int>(min(int64_t(32), a.M - row0));
-            for (int rr = 0; rr < rows; ++rr)
-              for (int c = lane; c < kCols; c += 32)
-                if (pc + c < a.N) {
-                  const int byte = c * static_cast<int>(sizeof(T));
-                  out[(row0 + rr) * a.N + pc + c] = *reinterpret_cast<const T*>(
-                      staging + rr * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
-                }
-          }
+        } else {
+          __syncwarp();
+          T* out = static_cast<T*>(a.out);
+          const int rows = static_cast<int>(min(int64_t(32), a.M - r0));
+          for (int rr = 0; rr < rows; ++rr)
+            for (int c = lane; c < kCols; c += 32)
+              if (pc + c < a.N) {
+                const int byte = c * static_cast<int>(sizeof(T));
+                out[static_cast<int64_t>(r0 + rr) * a.N + pc + c] =
+                    *reinterpret_cast<const T*>(stg + rr * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
+              }
+          __syncwarp();
         }
       }
     }
@@ -614,22 +695,41 @@ __global__ void __launch_bounds__(kSliceThreads)
     uint32_t r[32];
     tmem_ld_32x32b_x32(lane_base + c * 32, r);
     tmem_ld_wait_regs(r);
+    if (S > 1) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (c * 32 + j < cols) {
-        const float v = __uint_as_float(r[j]);
-        if (S > 1) part[(c * 32 + j) * 128 + threadIdx.x] = v;
-        else if (n < a.N) out[(c * 32 + j) * a.N] = from_f<T>(apply_act(v + bias, a.act));
-      }
+      for (int j = 0; j < 32; ++j)
+        if (c * 32 + j < cols) part[(c * 32 + j) * 128 + threadIdx.x] = __uint_as_float(r[j]);
+      continue;
+    }
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + bias;
+    apply_act(v, a.act);
+    if (n < a.N) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (c * 32 + j < cols) out[(c * 32 + j) * a.N] = from_f<T>(v[j]);
+    }
   }
   tc_fence_before();
   if (S > 1) {
     cluster_sync();
     const uint32_t mine = smem_addr(part) + threadIdx.x * 4;
-    for (int j = rank; j < cols; j += S) {
-      float v = 0.f;
-      for (int s = 0; s < S; ++s) v += cluster_load_f(cluster_map(mine + j * 512, static_cast<uint32_t>(s)));
-      if (n < a.N) out[j * a.N] = from_f<T>(apply_act(v + bias, a.act));
+    for (int j = rank; j < cols; j += 2 * S) {  // two rows at a time
+      const bool two = j + S < cols;
+      float v[2] = {0.f, 0.f};
+      for (int s = 0; s < S; ++s) {
+        const uint32_t from = cluster_map(mine + j * 512, static_cast<uint32_t>(s));
+        v[0] += cluster_load_f(from);
+        if (two) v[1] += cluster_load_f(from + S * 512);
+      }
+      v[0] += bias;
+      v[1] += bias;
+      apply_act(v, a.act);
+      if (n < a.N) {
+        out[j * a.N] = from_f<T>(v[0]);
+        if (two) out[(j + S) * a.N] = from_f<T>(v[1]);
+      }
     }
     cluster_sync();  // no CTA leaves while another reads its sums
   } else {
