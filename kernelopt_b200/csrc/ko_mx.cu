@@ -1,7 +1,7 @@
 // Microscaled quantisation, its inverse, the 4-bit weight layout, and the residual + root-mean-square norm whose output
 // can be microscaled in the same pass. Formats and layout: ko_mx.cuh.
 //
-// All of these read and write each byte once and compute a few operations per element, so HBM bounds them. Eight
+// All of these read and write each byte once; HBM bounds them where the instructions per element are kept few. Eight
 // consecutive elements belong to a lane, four lanes to a block of 32 and sixteen lanes to the 128 elements of a scale
 // word, so a block's largest magnitude is two shuffles and its four scales are written as one 32-bit word.
 #include <cmath>
@@ -16,59 +16,101 @@ using namespace komx;
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------------------------------------
-// Quantisation: half a warp takes the 128 elements of one scale word at a time. Items run over k tiles, then rows,
-// the rows that fill the last tile of 128 included (scale words 0, no codes).
+// Quantisation and its inverse: half a warp takes the 128 elements of a scale word of kRows neighbouring rows, all loads
+// before the arithmetic. Items run over k tiles, then row groups; the rows that fill the last tile of 128 are included in
+// quantisation (scale words 0, no codes).
 // ---------------------------------------------------------------------------------------------------------
+constexpr int kRows = 4;
+
+struct Item {
+  int64_t row;
+  uint32_t kt;
+  int lane16;
+};
+__device__ __forceinline__ bool item_of(int64_t items, uint32_t ktiles, Item& it) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
+  if (item >= items) return false;
+  const int64_t group = items <= 0xffffffffll ? static_cast<uint32_t>(item) / ktiles : item / ktiles;
+  it.row = group * kRows;
+  it.kt = static_cast<uint32_t>(item - group * ktiles);
+  it.lane16 = threadIdx.x & 15;
+  return true;
+}
+
 template <typename T, int FMT, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t K,
                                                             int64_t ldx, int64_t items, uint32_t ktiles,
                                                             int64_t code_pitch, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
-  if (item >= items) return;
-  const int64_t row = items <= 0xffffffffll ? static_cast<uint32_t>(item) / ktiles : item / ktiles;
-  const int64_t kt = item - row * ktiles;
-  uint8_t* word = scales + scale_word_offset(row, kt, ktiles);
-  if (row >= rows) {
-    if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(word) = 0u;
-    return;
-  }
-  float v[8];
-  load8<T, VEC>(x + row * ldx, kt * 128 + (threadIdx.x & 15) * 8, K, v);
-  quantize_group<FMT>(v, 0xffffu << (threadIdx.x & 16), codes + row * code_pitch, kt, word);
-}
-
-template <typename T, int FMT>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
-                                                              const uint8_t* __restrict__ scales, int64_t K,
-                                                              int64_t items, uint32_t ktiles, int64_t code_pitch,
-                                                              T* __restrict__ out, bool vec) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
-  if (item >= items) return;
-  const int64_t row = items <= 0xffffffffll ? static_cast<uint32_t>(item) / ktiles : item / ktiles;
-  const int64_t kt = item - row * ktiles;
-  const int lane16 = threadIdx.x & 15;
-  const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(scales + scale_word_offset(row, kt, ktiles)));
-  const float s = scale_value((word >> (8 * (lane16 >> 2))) & 255u);
-  const uint8_t* src = codes + row * code_pitch;
-  float v[8];
-  if constexpr (FMT == KO_MXFP4) {
-    unpack_e2m1x8(__ldg(reinterpret_cast<const uint32_t*>(src + kt * 64 + lane16 * 4)), v);
+  Item it;
+  if (!item_of(items, ktiles, it)) return;
+  uint8_t* word = scales + scale_word_offset(it.row, it.kt, ktiles);  // the group's rows are 16 bytes apart
+  const int real = static_cast<int>(min(int64_t(kRows), rows - it.row));
+  const int64_t k = static_cast<int64_t>(it.kt) * 128 + it.lane16 * 8;
+  const int left = static_cast<int>(K - k);
+  const T* p = x + it.row * ldx + k;
+  uint8_t* code = codes + it.row * code_pitch + static_cast<int64_t>(it.kt) * (FMT == KO_MXFP4 ? 64 : 128) +
+                  it.lane16 * (FMT == KO_MXFP4 ? 4 : 8);
+  Raw8<T> r[kRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= s;
-  } else {
-    const uint2 c = __ldg(reinterpret_cast<const uint2*>(src + kt * 128 + lane16 * 8));
+  for (int i = 0; i < kRows; ++i) r[i] = load8<T, VEC>(p + i * ldx, i < real ? left : 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack_e4m3x2(((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xffffu);
-      v[2 * i] = f.x * s;
-      v[2 * i + 1] = f.y * s;
+  for (int i = 0; i < kRows; ++i) {
+    if (i < real) {
+      float v[8];
+      widen8(r[i], v);
+      quantize_group<FMT>(v, amax_bits8(r[i]), 0xffffu << (threadIdx.x & 16), code + i * code_pitch, word + 16 * i);
+    } else if (it.lane16 == 0) {
+      *reinterpret_cast<uint32_t*>(word + 16 * i) = 0u;
     }
   }
-  T* dst = out + row * K;
-  const int64_t c0 = kt * 128 + lane16 * 8;
-  if (vec) store8<T, true>(dst, c0, K, v);
-  else store8<T, false>(dst, c0, K, v);
+}
+
+template <typename T, int FMT, bool VEC>
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
+                                                              const uint8_t* __restrict__ scales, int64_t rows,
+                                                              int64_t K, int64_t items, uint32_t ktiles,
+                                                              int64_t code_pitch, T* __restrict__ out) {
+  Item it;
+  if (!item_of(items, ktiles, it)) return;
+  const uint8_t* word = scales + scale_word_offset(it.row, it.kt, ktiles) + (it.lane16 >> 2);
+  const int real = static_cast<int>(min(int64_t(kRows), rows - it.row));
+  const int64_t k = static_cast<int64_t>(it.kt) * 128 + it.lane16 * 8;
+  const int left = static_cast<int>(K - k);
+  const uint8_t* code = codes + it.row * code_pitch + static_cast<int64_t>(it.kt) * (FMT == KO_MXFP4 ? 64 : 128) +
+                        it.lane16 * (FMT == KO_MXFP4 ? 4 : 8);
+  T* dst = out + it.row * K + k;
+  uint2 c[kRows];
+  uint32_t byte[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    c[i] = make_uint2(0u, 0u);
+    byte[i] = 0u;
+    if (i < real) {
+      byte[i] = __ldg(word + 16 * i);
+      if constexpr (FMT == KO_MXFP4) c[i].x = __ldg(reinterpret_cast<const uint32_t*>(code + i * code_pitch));
+      else c[i] = __ldg(reinterpret_cast<const uint2*>(code + i * code_pitch));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    if (i >= real) break;
+    const float s = scale_value(byte[i]);
+    float v[8];
+    if constexpr (FMT == KO_MXFP4) {
+      unpack_e2m1x8(c[i].x, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack_e4m3x2(((j < 2 ? c[i].x : c[i].y) >> (16 * (j & 1))) & 0xffffu);
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= s;
+    store8<T, VEC>(dst + i * K, left, v);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -128,92 +170,114 @@ struct NormArgs {
 template <typename T, int OUT, bool VEC, int TPR, int NV>
 __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kernel(const NormArgs a) {
   constexpr int kBlock = TPR > kThreads ? TPR : kThreads;
-  constexpr int kRows = kBlock / TPR;
+  constexpr int kBlockRows = kBlock / TPR;
   constexpr int kWarps = TPR / 32;  // warps of a row (0: half a warp)
   __shared__ float part[kBlock / 32];
   const int t = threadIdx.x % TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kBlockRows + threadIdx.x / TPR;
   const bool real = row < a.rows;
-  const int64_t C = a.C;
+  const int left = real ? static_cast<int>(a.C) - t * 8 : 0;  // elements from this thread's first one to the row's end
+  constexpr int kStep = TPR * 8;
   float v[NV][8];
-  float sum = 0.f;
-  if (real) {
-    const T* h = static_cast<const T*>(a.h) + row * a.ldh;
-    const T* o = a.o ? static_cast<const T*>(a.o) + row * a.ldo : nullptr;
+  {
+    const T* h = static_cast<const T*>(a.h) + row * a.ldh + t * 8;
+    Raw8<T> r[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t c = (t + i * TPR) * 8;
-      if (c >= C) {
+    for (int i = 0; i < NV; ++i) r[i] = load8<T, VEC>(h + i * kStep, left - i * kStep);
+    if (a.o) {
+      const T* o = static_cast<const T*>(a.o) + row * a.ldo + t * 8;
+      Raw8<T> q[NV];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-        continue;
-      }
-      load8<T, VEC>(h, c, C, v[i]);
-      if (o) {
-        float r[8];
-        load8<T, VEC>(o, c, C, r);
-        if (a.bias) {
+      for (int i = 0; i < NV; ++i) q[i] = load8<T, VEC>(o + i * kStep, left - i * kStep);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) widen8(q[i], v[i]);
+      if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
           float b[8];
-          load8<T, VEC>(static_cast<const T*>(a.bias), c, C, b);
+          widen8(load8<T, VEC>(static_cast<const T*>(a.bias) + t * 8 + i * kStep, left - i * kStep), b);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) r[j] += b[j];
+          for (int j = 0; j < 8; ++j) v[i][j] += b[j];
         }
-        if (a.scale) {
-          float s[8];
-          load8<T, VEC>(static_cast<const T*>(a.scale), c, C, s);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) r[j] *= s[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] += r[j];
       }
-      if (a.h_out) store8<T, VEC>(static_cast<T*>(a.h_out) + row * C, c, C, v[i]);
-    }
+      if (a.scale) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      sum += ((v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3])) +
-             ((v[i][4] * v[i][4] + v[i][5] * v[i][5]) + (v[i][6] * v[i][6] + v[i][7] * v[i][7]));
+        for (int i = 0; i < NV; ++i) {
+          float s[8];
+          widen8(load8<T, VEC>(static_cast<const T*>(a.scale) + t * 8 + i * kStep, left - i * kStep), s);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] *= s[j];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float x[8];
+        widen8(r[i], x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += x[j];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) widen8(r[i], v[i]);
+    }
   }
+  Raw8<T> g[NV];  // on its way while the sum is taken
+#pragma unroll
+  for (int i = 0; i < NV; ++i) g[i] = load8<T, VEC>(static_cast<const T*>(a.gamma) + t * 8 + i * kStep, left - i * kStep);
+  if (a.h_out) {
+    T* h_out = static_cast<T*>(a.h_out) + row * a.C + t * 8;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store8<T, VEC>(h_out + i * kStep, left - i * kStep, v[i]);
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    sum += ((v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3])) +
+           ((v[i][4] * v[i][4] + v[i][5] * v[i][5]) + (v[i][6] * v[i][6] + v[i][7] * v[i][7]));
 #pragma unroll
   for (int s = (TPR < 32 ? TPR : 32) / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   if constexpr (kWarps > 1) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
     __syncthreads();
     const int w0 = (threadIdx.x / TPR) * kWarps;
-    float p = (threadIdx.x & 31) < kWarps ? part[w0 + (threadIdx.x & 31)] : 0.f;
+    sum = (threadIdx.x & 31) < kWarps ? part[w0 + (threadIdx.x & 31)] : 0.f;
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) p += __shfl_xor_sync(0xffffffffu, p, s);
-    sum = p;
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   }
-  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(C) + a.eps);
-  if (row >= a.grid_rows) return;
+  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.C) + a.eps);
+  if constexpr (OUT < 0) {
+    if (!real) return;
+    T* y = static_cast<T*>(a.y) + row * a.C + t * 8;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t g = t + i * TPR;
-    const int64_t c = g * 8;
-    if constexpr (OUT < 0) {
-      if (real && c < C) {
-        float gm[8];
-        load8<T, VEC>(static_cast<const T*>(a.gamma), c, C, gm);
+    for (int i = 0; i < NV; ++i) {
+      float gm[8];
+      widen8(g[i], gm);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * gm[j];
-        store8<T, VEC>(static_cast<T*>(a.y) + row * C, c, C, v[i]);
+      for (int j = 0; j < 8; ++j) gm[j] *= v[i][j] * rstd;
+      store8<T, VEC>(y + i * kStep, left - i * kStep, gm);
+    }
+  } else {
+    if (row >= a.grid_rows) return;
+    uint8_t* word = a.scales + scale_word_offset(row, t >> 4, a.ktiles);  // a k tile is 512 bytes
+    constexpr int kBytes = OUT == KO_MXFP4 ? 4 : 8;
+    uint8_t* code = a.codes + row * a.code_pitch + t * kBytes;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if ((t >> 4) + i * (TPR / 16) >= static_cast<int>(a.ktiles)) break;  // the same for the sixteen lanes of a group
+      if (!real) {
+        if ((t & 15) == 0) *reinterpret_cast<uint32_t*>(word + i * (TPR / 16) * 512) = 0u;
+        continue;
       }
-    } else {
-      const int64_t kt = g >> 4;
-      if (kt < a.ktiles) {  // the same for the sixteen lanes of a group
-        uint8_t* word = a.scales + scale_word_offset(row, kt, a.ktiles);
-        if (!real) {
-          if ((t & 15) == 0) *reinterpret_cast<uint32_t*>(word) = 0u;
-        } else {
-          float gm[8];
-          load8<T, VEC>(static_cast<const T*>(a.gamma), c, C, gm);
-          // beyond C: v is 0 there and gm is 0; 0 * rstd would be NaN for an infinite rstd (eps 0, a row of zeros)
+      float gm[8];
+      widen8(g[i], gm);
+      // beyond C v is 0, and 0 * rstd would be NaN for an infinite rstd (eps 0, a row of zeros)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = c + j < C ? v[i][j] * rstd * gm[j] : 0.f;
-          quantize_group<OUT>(v[i], 0xffffu << (threadIdx.x & 16), a.codes + row * a.code_pitch, kt, word);
-        }
+      for (int j = 0; j < 8; ++j) {
+        gm[j] *= v[i][j] * rstd;
+        if (VEC ? left - i * kStep <= 0 : j >= left - i * kStep) gm[j] = 0.f;
       }
+      quantize_group<OUT>(gm, amax_bits8(gm), 0xffffu << (threadIdx.x & 16), code + i * TPR * kBytes,
+                          word + i * (TPR / 16) * 512);
     }
   }
 }
@@ -248,7 +312,7 @@ int dispatch_norm(const NormArgs& a, int out, bool vec, cudaStream_t s) {
 template <typename T, int FMT>
 int launch_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, void* codes, void* scales, bool vec,
                     cudaStream_t s) {
-  const int64_t ktiles = padded_k(K) / 128, items = (rows + 127) / 128 * 128 * ktiles;
+  const int64_t ktiles = padded_k(K) / 128, items = (rows + 127) / 128 * (128 / kRows) * ktiles;
   const int64_t blocks = (items + kThreads / 16 - 1) / (kThreads / 16);
   if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_quantize_mx: too many elements");
   const int64_t pitch = code_pitch(K, FMT);
@@ -266,18 +330,17 @@ int launch_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, void* c
 template <typename T>
 int launch_dequantize(const void* codes, const void* scales, int fmt, int64_t rows, int64_t K, void* out,
                       cudaStream_t s) {
-  const int64_t ktiles = padded_k(K) / 128, items = rows * ktiles;
+  const int64_t ktiles = padded_k(K) / 128, items = (rows + kRows - 1) / kRows * ktiles;
   const int64_t blocks = (items + kThreads / 16 - 1) / (kThreads / 16);
   if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_dequantize_mx: too many elements");
-  const bool vec = ko::aligned16(out) && (K * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+  const bool vec = reinterpret_cast<uintptr_t>(out) % (8 * sizeof(T)) == 0 && K % 8 == 0;
   const uint8_t *c = static_cast<const uint8_t*>(codes), *sc = static_cast<const uint8_t*>(scales);
-  const unsigned g = static_cast<unsigned>(blocks);
-  if (fmt == KO_MXFP4)
-    dequantize_kernel<T, KO_MXFP4><<<g, kThreads, 0, s>>>(c, sc, K, items, static_cast<uint32_t>(ktiles),
-                                                          code_pitch(K, fmt), static_cast<T*>(out), vec);
-  else
-    dequantize_kernel<T, KO_MXFP8><<<g, kThreads, 0, s>>>(c, sc, K, items, static_cast<uint32_t>(ktiles),
-                                                          code_pitch(K, fmt), static_cast<T*>(out), vec);
+  auto go = [&](auto kernel) {
+    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(c, sc, rows, K, items, static_cast<uint32_t>(ktiles),
+                                                              code_pitch(K, fmt), static_cast<T*>(out));
+  };
+  if (fmt == KO_MXFP4) go(vec ? dequantize_kernel<T, KO_MXFP4, true> : dequantize_kernel<T, KO_MXFP4, false>);
+  else go(vec ? dequantize_kernel<T, KO_MXFP8, true> : dequantize_kernel<T, KO_MXFP8, false>);
   return ko::check_launch("ko_dequantize_mx");
 }
 
@@ -305,7 +368,7 @@ extern "C" int ko_quantize_mx(const void* x, int dtype, int64_t rows, int64_t K,
   const int64_t es = dtype_size(dtype);
   if (!aligned_to(x, es) || !ko::aligned16(codes) || !ko::aligned16(scales))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "x must be aligned to its elements, codes and scales to 16 bytes");
-  const bool vec = ko::aligned16(x) && ldx * es % 16 == 0;
+  const bool vec = groups_of_8(x, dtype, ldx, K);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool f4 = fmt == KO_MXFP4;
   if (dtype == KO_F32)
@@ -380,11 +443,11 @@ extern "C" int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, in
   if (h_out == h && ldh != C)
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "h_out may be h only where h is contiguous");
   const int64_t es = dtype_size(dtype);
-  bool vec = ldh * es % 16 == 0 && (!o || ldo * es % 16 == 0) && C * es % 16 == 0;
+  bool vec = ldh % 8 == 0 && (!o || ldo % 8 == 0);
   const void* elems[] = {h, o, bias, scale, gamma, h_out, y};
   for (const void* p : elems) {
     if (p && !aligned_to(p, es)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "a pointer is not aligned to its elements");
-    vec = vec && ko::aligned16(p);
+    vec = vec && groups_of_8(p, dtype, C, C);
   }
   if (!y && (!ko::aligned16(codes) || !ko::aligned16(scales)))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "codes and scales must be 16-byte aligned");

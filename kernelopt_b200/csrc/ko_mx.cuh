@@ -20,6 +20,11 @@ inline int64_t code_pitch(int64_t K, int fmt) { return fmt == KO_MXFP4 ? padded_
 inline bool fmt_ok(int fmt) { return fmt == KO_MXFP4 || fmt == KO_MXFP8; }
 inline bool dtype_ok(int dt) { return dt == KO_F32 || dt == KO_BF16 || dt == KO_F16; }
 inline int64_t dtype_size(int dt) { return dt == KO_F32 ? 4 : 2; }
+// Whether rows of `dtype` at p, `pitch` elements apart and `width` long, are whole groups of eight that one access moves.
+inline bool groups_of_8(const void* p, int dtype, int64_t pitch, int64_t width) {
+  const int64_t group = 8 * dtype_size(dtype);
+  return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(group) == 0 && pitch % 8 == 0 && width % 8 == 0;
+}
 // Bounds that keep every size and offset product of these entry points inside 62 bits.
 constexpr int64_t kMaxRows = int64_t(1) << 31;
 constexpr int64_t kMaxK = int64_t(1) << 24;
@@ -36,82 +41,127 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-// Eight consecutive elements: 32 aligned bytes (fp32) or 16 (bf16, fp16).
-template <typename T> struct Vec8;
-template <> struct Vec8<float> {
-  float4 a, b;
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-    a = make_float4(v[0], v[1], v[2], v[3]);
-    b = make_float4(v[4], v[5], v[6], v[7]);
+// Eight consecutive elements as they lie in memory, moved by one access of 256 bits (fp32) or 128 (bf16, fp16). Two
+// 128-bit accesses of a lane's 32 bytes would each touch half of every 32-byte sector: the fp32 stores of 25600 x 1536
+// dequantised values took 43 us that way.
+template <typename T>
+struct alignas(16) Raw8 {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) w[i] = 0u;
   }
 };
-template <> struct __align__(16) Vec8<__nv_bfloat16> {
-  __nv_bfloat162 p[4];
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+__device__ __forceinline__ void widen8(const Raw8<float>& r, float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __bfloat1622float2(p[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[i]);
+}
+__device__ __forceinline__ void widen8(const Raw8<__nv_bfloat16>& r, float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-  }
-};
-template <> struct __align__(16) Vec8<__half> {
-  __half2 p[4];
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(p[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-  }
-};
-
-// Elements [c, c + 8) of a row of C, zero beyond C. VEC: the row starts on 16 bytes, so a whole group is one or two
-// 128-bit loads; otherwise, and in the group that C cuts, element by element.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t C, float (&v)[8]) {
-  if (VEC && c + 8 <= C) {
-    Vec8<T> t = *reinterpret_cast<const Vec8<T>*>(row + c);
-    t.get(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < C ? to_f(row[c + i]) : 0.f;
+  for (int i = 0; i < 4; ++i) {  // a bf16 is the upper half of its fp32
+    v[2 * i] = __uint_as_float(r.w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
   }
 }
+__device__ __forceinline__ void widen8(const Raw8<__half>& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> narrow8(const float (&v)[8]) {
+  Raw8<T> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+  }
+  return r;
+}
+
+// The group of eight elements at `p`, of which `left` (any integer) lie before the end of the row; the others are zero.
+// VEC: the row starts on a multiple of a group's bytes and its length is a multiple of 8, so a group is whole or beyond
+// the end.
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int64_t c, int64_t C, const float (&v)[8]) {
-  if (VEC && c + 8 <= C) {
-    Vec8<T> t;
-    t.set(v);
-    *reinterpret_cast<Vec8<T>*>(row + c) = t;
+__device__ __forceinline__ Raw8<T> load8(const T* p, int left) {
+  Raw8<T> r;
+  r.clear();
+  if (VEC) {
+    if (left > 0) {
+      if constexpr (sizeof(T) == 4) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                       "=r"(r.w[7])
+                     : "l"(p));
+      } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c + i < C) row[c + i] = from_f<T>(v[i]);
+      if (i < left) reinterpret_cast<T*>(r.w)[i] = p[i];
+  }
+  return r;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
+  if (VEC) {
+    if (left > 0) {
+      const Raw8<T> r = narrow8<T>(v);
+      if constexpr (sizeof(T) == 4)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]),
+                     "r"(r.w[2]), "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7])
+                     : "memory");
+      else
+        *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = from_f<T>(v[i]);
   }
 }
 
 // Largest magnitude of eight values as the bits of an fp32: ordered like the magnitudes, with infinity and then NaN
-// above every finite value, so that one integer maximum also finds what is not finite.
+// above every finite value, so that one integer maximum also finds what is not finite. The 16-bit types are compared two
+// at a time in their own bits, which are ordered the same way.
 __device__ __forceinline__ uint32_t amax_bits8(const float (&v)[8]) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
   return m;
+}
+__device__ __forceinline__ uint32_t amax_bits8(const Raw8<float>& r) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, r.w[i] & 0x7fffffffu);
+  return m;
+}
+__device__ __forceinline__ uint32_t amax_pairs(const uint32_t (&w)[4]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return max(m >> 16, m & 0xffffu);
+}
+__device__ __forceinline__ uint32_t amax_bits8(const Raw8<__nv_bfloat16>& r) { return amax_pairs(r.w) << 16; }
+__device__ __forceinline__ uint32_t amax_bits8(const Raw8<__half>& r) {
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(amax_pairs(r.w)))));
 }
 // The block's e8m0 byte: floor(log2(amax)) - emax + 127, held to 0 or above; 255 (NaN) where amax is not finite. The
 // exponent field of amax is floor(log2) + 127 for a normal number, and both subnormals and zero end at byte 0.
@@ -189,31 +239,30 @@ __device__ __forceinline__ int64_t scale_word_offset(int64_t row, int64_t ktile,
   return ((row >> 7) * ktiles + ktile) * 512 + (r & 31) * 16 + (r >> 5) * 4;
 }
 
-// Writes the codes of a lane's eight values and, from one lane in sixteen, the scale word of their 128 elements.
-// Every group of sixteen lanes that calls this together holds one row's elements [128 kt, 128 kt + 128) in order;
-// `mask` names the calling lanes.
+// Writes the codes of a lane's eight values and, from one lane in sixteen, the scale word of their 128 elements. A group
+// of sixteen lanes that calls this together holds one row's elements [128 kt, 128 kt + 128) in order; `mask` names them, m
+// is the largest magnitude of the lane's own values, `code` the address of their codes.
 template <int FMT>
-__device__ __forceinline__ void quantize_group(const float (&v)[8], uint32_t mask, uint8_t* __restrict__ code_row,
-                                               int64_t kt, uint8_t* __restrict__ scale_word) {
+__device__ __forceinline__ void quantize_group(const float (&v)[8], uint32_t m, uint32_t mask, uint8_t* code,
+                                               uint8_t* scale_word) {
   const int lane16 = threadIdx.x & 15;
-  uint32_t m = amax_bits8(v);
   m = max(m, __shfl_xor_sync(mask, m, 1));
   m = max(m, __shfl_xor_sync(mask, m, 2));
   const uint32_t byte = scale_byte<FMT>(m);
   const float inv = scale_inverse(byte);
+  // a NaN or an infinity times the zero inverse is NaN, which would convert to the largest code: such blocks are cleared
   if constexpr (FMT == KO_MXFP4) {
-    // a NaN or an infinity times the zero inverse is NaN, which would convert to the largest code
-    const uint32_t c = byte == 255u ? 0u : pack_e2m1x8(v, inv);
-    *reinterpret_cast<uint32_t*>(code_row + kt * 64 + lane16 * 4) = c;
+    const uint32_t c = pack_e2m1x8(v, inv);
+    *reinterpret_cast<uint32_t*>(code) = byte == 255u ? 0u : c;
   } else {
     uint2 c = pack_e4m3x8(v, inv);
     if (byte == 255u) c = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2*>(code_row + kt * 128 + lane16 * 8) = c;
+    *reinterpret_cast<uint2*>(code) = c;
   }
-  uint32_t w = byte << (8 * (lane16 >> 2));
-  w |= __shfl_xor_sync(mask, w, 4);
-  w |= __shfl_xor_sync(mask, w, 8);
-  if (lane16 == 0) *reinterpret_cast<uint32_t*>(scale_word) = w;
+  // bytes of lanes 0, 4, 8, 12 into lane 0's word
+  const uint32_t pair = byte | (__shfl_down_sync(mask, byte, 4, 16) << 8);
+  const uint32_t word = pair | (__shfl_down_sync(mask, pair, 8, 16) << 16);
+  if (lane16 == 0) *reinterpret_cast<uint32_t*>(scale_word) = word;
 }
 
 #endif  // __CUDACC__

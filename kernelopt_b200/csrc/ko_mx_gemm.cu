@@ -176,16 +176,6 @@ __device__ __forceinline__ void apply_act(float (&v)[N], int act) {
   }
 }
 
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 p = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-
 // ---------------------------------------------------------------------------------------------------------
 // pair_kernel: persistent CTA pairs (clusters of two), 256 x 256 output tiles. The pair's tensor cores run as one
 // (cta_group::2): each CTA holds 128 rows of A and 128 of the 256 weight rows of a stage and receives its 128 x 256 half
@@ -515,19 +505,24 @@ struct SliceArgs {
   int act, k_stages, n_tiles, slices;
   const void* x;  // unquantised rows [M][K], ldx elements apart (XT other than void)
   int64_t K, ldx;
-  int x_vec;      // rows of x start on 16 bytes
+  int x_vec;      // rows of x are whole groups of eight (groups_of_8)
 };
 
 // A block of 32 elements from k on, zero beyond K: its mxfp4 codes and its scale byte.
 template <typename XT>
 __device__ __forceinline__ uint4 quantize_block(const XT* row, int64_t k, int64_t K, bool vec, uint32_t& byte) {
-  float v[4][8];
+  Raw8<XT> r[4];
   uint32_t m = 0;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    if (vec) load8<XT, true>(row, k + g * 8, K, v[g]);
-    else load8<XT, false>(row, k + g * 8, K, v[g]);
-    m = max(m, amax_bits8(v[g]));
+    const int left = static_cast<int>(K - k) - g * 8;
+    r[g] = vec ? load8<XT, true>(row + k + g * 8, left) : load8<XT, false>(row + k + g * 8, left);
+  }
+  float v[4][8];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    m = max(m, amax_bits8(r[g]));
+    widen8(r[g], v[g]);
   }
   byte = scale_byte<KO_MXFP4>(m);
   if (byte == 255u) return make_uint4(0u, 0u, 0u, 0u);
@@ -896,7 +891,7 @@ int launch_slice(const Call& c) {
     a.x = c.x;
     a.K = c.K;
     a.ldx = c.ldx;
-    a.x_vec = ko::aligned16(c.x) && c.ldx * static_cast<int64_t>(sizeof(XT)) % 16 == 0;
+    a.x_vec = reinterpret_cast<uintptr_t>(c.x) % (8 * sizeof(XT)) == 0 && c.ldx % 8 == 0 && c.K % 8 == 0;
   }
   a.bias = c.bias;
   a.out = c.out;
