@@ -10,8 +10,8 @@
 // scales of 128 rows x 128 elements are one 512-byte tile in HBM; TMA brings the stage's tiles in and tcgen05.cp spreads
 // them over tensor memory, ahead of the stage's MMAs on the same pipe.
 //
-// Two kernels: pairs of CTAs with 256 x 256 tiles for many rows (pair_kernel), and single CTAs over slices of K for few
-// (slice_kernel). Every wait is bounded; a wait that runs out ends the kernel with KO_ERR_DEVICE_TIMEOUT in *dev_status.
+// Two kernels: pairs of CTAs with tiles of 256 rows for many rows (pair_kernel), and single CTAs over slices of K for few
+// (slice_kernel); launch() says which takes a product. Every wait is bounded; a wait that runs out ends the kernel with KO_ERR_DEVICE_TIMEOUT in *dev_status.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -95,14 +95,19 @@ __device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_
       "l"(map), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
-__device__ __forceinline__ float cluster_load_f(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 cluster_load_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
-__device__ __forceinline__ bool wait_cluster_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  const bool ok = mbar_wait_cluster(bar, parity, abort);
-  return __all_sync(0xffffffffu, ok);
+// Arrive on a barrier of the pair's leader. What the arrival orders are tensor-memory reads, before the MMAs that the leader
+// issues next, and the tcgen05 fences on both sides see to that; a release at cluster scope, a memory barrier across the
+// pair, made each tile's hand-over a microsecond longer.
+__device__ __forceinline__ void arrive_leader(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 template <bool F4>
@@ -177,36 +182,40 @@ __device__ __forceinline__ void apply_act(float (&v)[N], int act) {
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// pair_kernel: persistent CTA pairs (clusters of two), 256 x 256 output tiles. The pair's tensor cores run as one
-// (cta_group::2): each CTA holds 128 rows of A and 128 of the 256 weight rows of a stage and receives its 128 x 256 half
-// of the product in its own tensor memory, so an SM loads 32 KB of codes per stage for twice the work of a 128 x 128 tile.
+// pair_kernel: persistent CTA pairs (clusters of two), 256 x BN output tiles. The pair's tensor cores run as one
+// (cta_group::2): each CTA holds 128 rows of A and half of the BN weight rows of a stage and receives its 128 x BN half of
+// the product in its own tensor memory, so an SM loads less per MMA than with tiles of its own.
 //   warp 0       TMA producer of this CTA; its bytes count on the leader's `full` barrier
 //   warp 1       tensor memory; in the leader it copies the scales and issues the MMAs of both CTAs
-//   warps 2-17   epilogue: per lane quarter four warps of 64 columns each; accumulator -> + bias, activation, one rounding
-//                -> a swizzled tile in shared memory -> TMA store (rows of `out` on 16 bytes), or element stores (other N)
-// Tensor memory (512 columns): two accumulators of 256 columns that share [128, 256), the scales in [384, 512) with a slot
-// per stage. Warps 2-9 read the shared half into registers and then let the next tile's MMAs go; warps 10-17 have until
-// the tile after it for the other half. So all but the read of half an accumulator overlaps the MMAs.
+//   warps 2-17   epilogue, 64 columns of a lane quarter each: accumulator -> + bias, activation, one rounding -> a
+//                swizzled tile in shared memory -> TMA store (rows of `out` on 16 bytes), or element stores (other N)
+// Tensor memory (512 columns): the accumulators in [0, 384), the scales in [384, 512) with a slot per stage.
+//   BN 256: two accumulators that share [128, 256). Warps 2-9 read the shared half into registers and then let the next
+//           tile's MMAs go; warps 10-17 have until the tile after it for the other half.
+//   BN 128: three accumulators; warps 2-9 take the even tiles and warps 10-17 the odd ones, so the MMAs run up to three
+//           tiles ahead.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kPairThreads = 18 * 32;
-constexpr int kPairTile = 256;
 
-template <bool F4>
+template <bool F4, int BN>
 struct PairCfg {
-  static constexpr int kStages = 4;
-  static constexpr uint32_t kOperand = 128 * 128;
-  static constexpr uint32_t kSfa = 512 * Elem<F4>::kKt, kSfb = 2 * kSfa;
-  static constexpr uint32_t kOffSf = 2 * kOperand;
-  static constexpr uint32_t kStage = (2 * kOperand + kSfa + kSfb + 1023) / 1024 * 1024;
-  static constexpr uint32_t kTx = 2 * (kOperand + Elem<F4>::kTxW + kSfa + kSfb);  // both CTAs
+  static constexpr int kStages = BN == 256 ? 4 : 6;  // what fits beside the staging tiles
+  static constexpr uint32_t kA = 128 * 128, kW = BN / 2 * 128;
+  static constexpr uint32_t kSfa = 512 * Elem<F4>::kKt, kSfw = BN / 128 * kSfa;
+  static constexpr uint32_t kOffSf = kA + kW;
+  static constexpr uint32_t kStage = (kOffSf + kSfa + kSfw + 1023) / 1024 * 1024;
+  static constexpr uint32_t kTx = 2 * (kA + Elem<F4>::kTxW * BN / 256 + kSfa + kSfw);  // both CTAs
   static constexpr uint32_t kOffStaging = kStages * kStage;
   static constexpr uint32_t kStaging = 32 * 128;  // 32 rows of 128 bytes for each epilogue warp
   static constexpr uint32_t kOffBias = kOffStaging + 16 * kStaging;  // 64 columns for each epilogue warp
   static constexpr uint32_t kOffBars = kOffBias + 16 * 64 * 4;
   static constexpr uint32_t kSmem = 1024 + kOffBars + 256;
-  static constexpr uint32_t kColSf = 384, kSfCols = 12 * Elem<F4>::kKt;  // per slot: A 4, W 8 per scale tile along K
+  static constexpr int kAccs = BN == 256 ? 2 : 3;                // accumulators, 128 columns apart
+  static constexpr uint32_t kSfwCols = 4 * (BN / 128);
+  static constexpr uint32_t kColSf = 384, kSfCols = (4 + kSfwCols) * Elem<F4>::kKt;  // a slot
+  static_assert(BN == 128 || BN == 256, "tile width");
   static_assert(kColSf + kStages * kSfCols <= 512, "tensor memory");
-  static_assert((2 * kStages + 6) * 8 + 16 <= 256, "barrier area");
+  static_assert((2 * kStages + 2 * kAccs + 2) * 8 + 16 <= 256, "barrier area");
 };
 
 struct PairArgs {
@@ -217,24 +226,25 @@ struct PairArgs {
   int act, k_stages, m_tiles, n_tiles, n_pairs, tma_out;
 };
 
-template <bool F4, typename T>
+template <bool F4, int BN, typename T>
 __global__ void __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                 const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sw,
                 const __grid_constant__ CUtensorMap map_out, const PairArgs a) {
-  using C = PairCfg<F4>;
+  using C = PairCfg<F4, BN>;
   using E = Elem<F4>;
+  constexpr int NA = C::kAccs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);  // stage landed in both CTAs (leader: 1 + tx)
   uint64_t* empty = full + C::kStages;    // stage's MMAs done            (1 commit, both CTAs)
-  // A barrier's parity cannot tell a phase from the one after the next, so where a waiter may be two tiles behind the last
-  // arrival there is a barrier for even tiles and one for odd.
-  uint64_t* acc_full = empty + C::kStages;  // tile's MMAs done           (1 commit, both CTAs) x 2
-  uint64_t* own_free = acc_full + 2;      // unshared half read           (8 warps x 2 CTAs, leader) x 2
-  uint64_t* shared_free = acc_full + 4;   // shared half read             (8 warps x 2 CTAs, leader)
-  uint64_t* mma_done = acc_full + 5;      // every MMA done               (1 commit, both CTAs)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 6);
+  // A barrier's parity cannot tell a phase from the one after the next, so every accumulator has barriers of its own: the
+  // waiters of one are never two of its tiles behind.
+  uint64_t* acc_full = empty + C::kStages;  // tile's MMAs done           (1 commit, both CTAs) x NA
+  uint64_t* acc_free = acc_full + NA;     // read, but for a shared half  (8 warps x 2 CTAs, leader) x NA
+  uint64_t* shared_free = acc_free + NA;  // shared half read             (8 warps x 2 CTAs, leader)
+  uint64_t* mma_done = shared_free + 1;   // every MMA done               (1 commit, both CTAs)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -254,10 +264,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&acc_full[0], 1);
-    mbar_init(&acc_full[1], 1);
-    mbar_init(&own_free[0], 16);
-    mbar_init(&own_free[1], 16);
+    for (int i = 0; i < NA; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_free[i], 16);
+    }
     mbar_init(shared_free, 16);
     mbar_init(mma_done, 1);
     *abort_flag = 0;
@@ -295,11 +305,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           uint8_t* s = smem + st * C::kStage;
           const uint32_t bar = leader_full + st * 8;
           if (rank == 0) mbar_arrive_expect_tx(&full[st], C::kTx);
-          const int half = static_cast<int>(rank) * 128;
-          tma_load_2d_pair(&map_a, bar, s, ks * 128, mt * 256 + half);
-          tma_load_2d_pair(&map_w, bar, s + C::kOperand, ks * 128, nt * 256 + half);
-          tma_load_2d_pair(&map_sa, bar, s + C::kOffSf, ks * 64 * E::kKt, mt * 2 + static_cast<int>(rank));
-          tma_load_2d_pair(&map_sw, bar, s + C::kOffSf + C::kSfa, ks * 64 * E::kKt, nt * 2);
+          const int r = static_cast<int>(rank);
+          tma_load_2d_pair(&map_a, bar, s, ks * 128, mt * 256 + r * 128);
+          tma_load_2d_pair(&map_w, bar, s + C::kA, ks * 128, nt * BN + r * (BN / 2));
+          tma_load_2d_pair(&map_sa, bar, s + C::kOffSf, ks * 64 * E::kKt, mt * 2 + r);
+          tma_load_2d_pair(&map_sw, bar, s + C::kOffSf + C::kSfa, ks * 64 * E::kKt, nt * (BN / 128));
           if (++st == C::kStages) {
             st = 0;
             phase ^= 1u;
@@ -313,36 +323,37 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      constexpr uint32_t idesc = idesc_bs(E::kTypeA, E::kTypeW, 256, 256);
+      constexpr uint32_t idesc = idesc_bs(E::kTypeA, E::kTypeW, 256, BN);
       const uint32_t sb = smem_addr(smem);
       int st = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; t < total && ok; t += a.n_pairs, ++local) {
-        // the previous tile's shared half, and the other half of the tile before it
-        if (local > 0 && !wait_cluster_warp(shared_free, static_cast<uint32_t>(local - 1) & 1u, abort_flag)) break;
-        if (local > 1 && !wait_cluster_warp(&own_free[local & 1], static_cast<uint32_t>((local >> 1) - 1) & 1u, abort_flag))
+        const int buf = local % NA, use = local / NA;  // this tile's accumulator, and the tiles before it there
+        if (BN == 256 && local > 0 && !mbar_wait_warp(shared_free, static_cast<uint32_t>(local - 1) & 1u, abort_flag))
           break;
+        if (use > 0 && !mbar_wait_warp(&acc_free[buf], static_cast<uint32_t>(use - 1) & 1u, abort_flag)) break;
         tc_fence_after();
-        const uint32_t d = tmem + (local & 1) * 128;
+        const uint32_t d = tmem + buf * 128;
         for (int ks = 0; ks < a.k_stages; ++ks) {
-          if (!wait_cluster_warp(&full[st], phase, abort_flag)) {
+          if (!mbar_wait_warp(&full[st], phase, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t s = sb + st * C::kStage;
-          const uint32_t sfa = tmem + C::kColSf + st * C::kSfCols, sfb = sfa + 4 * E::kKt;
+          const uint32_t sfa = tmem + C::kColSf + st * C::kSfCols, sfw = sfa + 4 * E::kKt;
 #pragma unroll
           for (int kt = 0; kt < E::kKt; ++kt) {
             cp_scales_w<2>(sfa + 4 * kt, scale_desc(s + C::kOffSf + kt * 512));
-            cp_scales_w<2>(sfb + 8 * kt, scale_desc(s + C::kOffSf + C::kSfa + kt * 512));
-            cp_scales_w<2>(sfb + 8 * kt + 4, scale_desc(s + C::kOffSf + C::kSfa + (E::kKt + kt) * 512));
+#pragma unroll
+            for (int i = 0; i < BN / 128; ++i)
+              cp_scales_w<2>(sfw + C::kSfwCols * kt + 4 * i, scale_desc(s + C::kOffSf + C::kSfa + (i * E::kKt + kt) * 512));
           }
 #pragma unroll
           for (int j = 0; j < E::kMma; ++j)
-            mma_bs_w<2, F4>(d, smem_desc_k_sw128(s + j * 32), smem_desc_k_sw128(s + C::kOperand + j * 32),
-                            idesc | idesc_sf(E::sf_of(j)), sfa + 4 * E::kt_of(j), sfb + 8 * E::kt_of(j),
+            mma_bs_w<2, F4>(d, smem_desc_k_sw128(s + j * 32), smem_desc_k_sw128(s + C::kA + j * 32),
+                            idesc | idesc_sf(E::sf_of(j)), sfa + 4 * E::kt_of(j), sfw + C::kSfwCols * E::kt_of(j),
                             (ks > 0 || j > 0) ? 1u : 0u);
           mma_commit_pair_w(&empty[st]);
           if (++st == C::kStages) {
@@ -350,7 +361,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             phase ^= 1u;
           }
         }
-        if (ok) mma_commit_pair_w(&acc_full[local & 1]);
+        if (ok) mma_commit_pair_w(&acc_full[buf]);
       }
       mma_commit_pair_w(mma_done);
     }
@@ -358,61 +369,87 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (!mbar_wait_warp(mma_done, 0, &never)) *abort_flag = 1;
   } else {
     const int e = warp - 2, q = warp & 3;
-    const bool shared_half = e < 8;
-    const int h = (e >> 2) & 1;  // which 64 columns of the half
+    const int set = e >> 3;      // BN 256: the shared half of every tile or the other one; BN 128: even or odd tiles
+    const int h = (e >> 2) & 1;  // which 64 columns of the 128
+    constexpr int kEvery = BN == 256 ? 1 : 2;  // this warp's tiles among the pair's
     uint8_t* stg = smem + C::kOffStaging + e * C::kStaging;
     float* bias = reinterpret_cast<float*>(smem + C::kOffBias) + e * 64;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
-    const uint32_t free_bar = cluster_map(smem_addr(shared_half ? shared_free : own_free), 0);
+    const uint32_t free_bars = cluster_map(smem_addr(acc_free), 0);
     constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a staging row
-    // first tensor-memory column and first column of the output of this warp's part of tile t (the local-th)
+    // first tensor-memory column and first row and column of the output of this warp's part of tile t (the local-th)
     auto part_of = [&](int t, int local, int& col, int& row0, int& col0) {
       int mt, nt;
       tile_at(t, mt, nt);
-      col = (shared_half ? 128 : (local & 1) ? 256 : 0) + h * 64;
       row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32;
-      col0 = nt * 256 + col - (local & 1) * 128;
+      if (BN == 256) {
+        col = (set == 0 ? 128 : (local & 1) ? 256 : 0) + h * 64;
+        col0 = nt * 256 + col - (local & 1) * 128;
+      } else {
+        col = local % NA * 128 + h * 64;
+        col0 = nt * 128 + h * 64;
+      }
     };
     auto load_bias = [&](int col0, float& b0, float& b1) {  // columns 2 lane and 2 lane + 1
       const int n = col0 + 2 * lane;
       b0 = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
       b1 = a.bias && n + 1 < a.N ? __ldg(a.bias + n + 1) : 0.f;
     };
-    int local = 0, col, row0, col0;
-    part_of(pair, 0, col, row0, col0);
-    float b0, b1;
-    load_bias(col0, b0, b1);
-    for (int t = pair; t < total; t += a.n_pairs, ++local) {
+    int local = BN == 256 ? 0 : set, col = 0, row0 = 0, col0 = 0;
+    int t = pair + local * a.n_pairs;
+    float b0 = 0.f, b1 = 0.f;
+    if (t < total) {
+      part_of(t, local, col, row0, col0);
+      load_bias(col0, b0, b1);
+    }
+    for (; t < total; t += kEvery * a.n_pairs, local += kEvery) {
       __syncwarp();
       *reinterpret_cast<float2*>(bias + 2 * lane) = make_float2(b0, b1);
       __syncwarp();
       const int tcol = col, r0 = row0, c0 = col0;
-      if (t + a.n_pairs < total) {  // the next tile's bias comes while this tile is worked on
-        part_of(t + a.n_pairs, local + 1, col, row0, col0);
+      if (t + kEvery * a.n_pairs < total) {  // the next tile's bias comes while this tile is worked on
+        part_of(t + kEvery * a.n_pairs, local + kEvery, col, row0, col0);
         load_bias(col0, b0, b1);
       }
-      if (!mbar_wait_warp(&acc_full[local & 1], static_cast<uint32_t>(local >> 1) & 1u, abort_flag)) break;
+      if (!mbar_wait_warp(&acc_full[local % NA], static_cast<uint32_t>(local / NA) & 1u, abort_flag)) break;
       tc_fence_after();
-      uint32_t r[2][32];
-      tmem_ld_32x32b_x32(lane_base + tcol, r[0]);
-      tmem_ld_32x32b_x32(lane_base + tcol + 32, r[1]);
-      tmem_ld_wait_regs(r[0]);
-      tmem_ld_wait_regs(r[1]);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(free_bar + (shared_half ? 0 : (local & 1) * 8));
-      if (r0 >= a.M || c0 >= a.N) continue;
+      // BN 256: both chunks at once, for the next tile's MMAs wait on the shared half. BN 128: one after the other, which
+      // leaves registers for more of the activation at a time.
+      constexpr bool kBoth = BN == 256;
+      uint32_t r[kBoth ? 2 : 1][32];
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader(free_bars + (BN == 256 && set == 0 ? NA : local % NA) * 8);
+      };
+      if (kBoth) {
+        tmem_ld_32x32b_x32(lane_base + tcol, r[0]);
+        tmem_ld_32x32b_x32(lane_base + tcol + 32, r[kBoth ? 1 : 0]);
+        tmem_ld_wait_regs(r[0]);
+        tmem_ld_wait_regs(r[kBoth ? 1 : 0]);
+        release();
+      }
+      if (r0 >= a.M || c0 >= a.N) {
+        if (!kBoth) release();
+        continue;
+      }
       constexpr bool kWide = sizeof(T) == 4;  // 32 columns fill a staging row, else all 64 do
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        const uint32_t(&rc)[32] = r[kBoth ? c : 0];
+        if (!kBoth) {
+          tmem_ld_32x32b_x32(lane_base + tcol + c * 32, r[0]);
+          tmem_ld_wait_regs(r[0]);
+          if (c == 1) release();
+        }
         float v[32];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float4 b = reinterpret_cast<const float4*>(bias)[c * 8 + j];
-          v[4 * j] = __uint_as_float(r[c][4 * j]) + b.x;
-          v[4 * j + 1] = __uint_as_float(r[c][4 * j + 1]) + b.y;
-          v[4 * j + 2] = __uint_as_float(r[c][4 * j + 2]) + b.z;
-          v[4 * j + 3] = __uint_as_float(r[c][4 * j + 3]) + b.w;
+          v[4 * j] = __uint_as_float(rc[4 * j]) + b.x;
+          v[4 * j + 1] = __uint_as_float(rc[4 * j + 1]) + b.y;
+          v[4 * j + 2] = __uint_as_float(rc[4 * j + 2]) + b.z;
+          v[4 * j + 3] = __uint_as_float(rc[4 * j + 3]) + b.w;
         }
         apply_act(v, a.act);
         if (kWide || c == 0) {
@@ -503,6 +540,7 @@ struct SliceArgs {
   int* dev_status;
   int64_t M, N;
   int act, k_stages, n_tiles, slices;
+  int vec_out;    // four neighbours of a row of out can be stored at once
   const void* x;  // unquantised rows [M][K], ldx elements apart (XT other than void)
   int64_t K, ldx;
   int x_vec;      // rows of x are whole groups of eight (groups_of_8)
@@ -528,6 +566,56 @@ __device__ __forceinline__ uint4 quantize_block(const XT* row, int64_t k, int64_
   if (byte == 255u) return make_uint4(0u, 0u, 0u, 0u);
   const float inv = scale_inverse(byte);
   return make_uint4(pack_e2m1x8(v[0], inv), pack_e2m1x8(v[1], inv), pack_e2m1x8(v[2], inv), pack_e2m1x8(v[3], inv));
+}
+
+// Adds the S partial sums of rows rank, rank + S, ... of a tile and stores them. A warp takes 8 / S rows at a time and a lane
+// four columns of them: eight 128-bit reads through distributed shared memory on their way at once, added in rank order.
+template <int S, typename T>
+__device__ __forceinline__ void add_slices(const SliceArgs& a, float* part, int nt, int64_t m0, int cols, int rank) {
+  constexpr int R = 8 / S;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n = static_cast<int64_t>(nt) * 128 + lane * 4;
+  uint32_t from[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) from[s] = cluster_map(smem_addr(part) + lane * 16, static_cast<uint32_t>(s));
+  float bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bias[i] = a.bias && n + i < a.N ? __ldg(a.bias + n + i) : 0.f;
+  for (int j0 = rank + S * R * warp; j0 < cols; j0 += S * R * (kSliceThreads / 32)) {
+    float4 p[R][S];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        p[r][s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j0 + r * S < cols) p[r][s] = cluster_load_f4(from[s] + (j0 + r * S) * 512);
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int j = j0 + r * S;
+      if (j >= cols) break;
+      float v[4] = {p[r][0].x, p[r][0].y, p[r][0].z, p[r][0].w};
+#pragma unroll
+      for (int s = 1; s < S; ++s) {
+        v[0] += p[r][s].x;
+        v[1] += p[r][s].y;
+        v[2] += p[r][s].z;
+        v[3] += p[r][s].w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += bias[i];
+      apply_act(v, a.act);
+      T* o = static_cast<T*>(a.out) + (m0 + j) * a.N + n;
+      if (n + 4 <= a.N && a.vec_out) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < a.N) o[i] = from_f<T>(v[i]);
+      }
+    }
+  }
 }
 
 template <bool F4, int BN, typename T, typename XT>
@@ -709,22 +797,10 @@ __global__ void __launch_bounds__(kSliceThreads)
   tc_fence_before();
   if (S > 1) {
     cluster_sync();
-    const uint32_t mine = smem_addr(part) + threadIdx.x * 4;
-    for (int j = rank; j < cols; j += 2 * S) {  // two rows at a time
-      const bool two = j + S < cols;
-      float v[2] = {0.f, 0.f};
-      for (int s = 0; s < S; ++s) {
-        const uint32_t from = cluster_map(mine + j * 512, static_cast<uint32_t>(s));
-        v[0] += cluster_load_f(from);
-        if (two) v[1] += cluster_load_f(from + S * 512);
-      }
-      v[0] += bias;
-      v[1] += bias;
-      apply_act(v, a.act);
-      if (n < a.N) {
-        out[j * a.N] = from_f<T>(v[0]);
-        if (two) out[(j + S) * a.N] = from_f<T>(v[1]);
-      }
+    switch (S) {
+      case 2: add_slices<2, T>(a, part, nt, m0, cols, rank); break;
+      case 4: add_slices<4, T>(a, part, nt, m0, cols, rank); break;
+      default: add_slices<8, T>(a, part, nt, m0, cols, rank); break;
     }
     cluster_sync();  // no CTA leaves while another reads its sums
   } else {
@@ -814,20 +890,20 @@ cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* attr, unsigned cluster, u
   return cfg;
 }
 
-template <bool F4, typename T>
+template <bool F4, int BN, typename T>
 int launch_pair(const Call& c) {
-  using C = PairCfg<F4>;
+  using C = PairCfg<F4, BN>;
   using E = Elem<F4>;
   constexpr const char* who = "ko_linear_mxfp4";
-  const int64_t mt = (c.M + kPairTile - 1) / kPairTile, nt = (c.N + kPairTile - 1) / kPairTile;
+  const int64_t mt = (c.M + 255) / 256, nt = (c.N + BN - 1) / BN;
   if (mt * nt > INT32_MAX / 16) return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(who) + ": too many output tiles");
   CUtensorMap ma, mw, msa, msw, mo;
   const int64_t es = static_cast<int64_t>(sizeof(T));
   const bool tma_out = ko::aligned16(c.out) && c.N * es % 16 == 0;
   int rc = encode_codes(&ma, c.ac, F4 ? KO_MXFP4 : KO_MXFP8, false, c.M, c.Kp, 128, who);
-  if (!rc) rc = encode_codes(&mw, c.wc, KO_MXFP4, !F4, c.N, c.Kp, 128, who);
+  if (!rc) rc = encode_codes(&mw, c.wc, KO_MXFP4, !F4, c.N, c.Kp, BN / 2, who);
   if (!rc) rc = encode_scales(&msa, c.as, c.M, c.Kp, E::kKt, 1, who);
-  if (!rc) rc = encode_scales(&msw, c.ws, c.N, c.Kp, E::kKt, 2, who);
+  if (!rc) rc = encode_scales(&msw, c.ws, c.N, c.Kp, E::kKt, BN / 128, who);
   mo = ma;  // not used without tma_out
   if (!rc && tma_out)
     rc = encode_2d(&mo, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, c.out, c.N, c.M,
@@ -844,7 +920,7 @@ int launch_pair(const Call& c) {
   a.m_tiles = static_cast<int>(mt);
   a.n_tiles = static_cast<int>(nt);
   a.tma_out = tma_out ? 1 : 0;
-  auto kernel = pair_kernel<F4, T>;
+  auto kernel = pair_kernel<F4, BN, T>;
   static std::atomic<bool> allowed[kMaxDevices];
   static std::atomic<int> resident[kMaxDevices];  // CTA pairs that the device holds at once, found once per device
   const int dev = current_device();
@@ -904,6 +980,7 @@ int launch_slice(const Call& c) {
   int slices = 1;
   while (slices < 8 && mt * nt * slices * 2 <= 2 * c.info->sm_count && slices * 2 <= a.k_stages) slices *= 2;
   a.slices = slices;
+  a.vec_out = c.N % 4 == 0 && reinterpret_cast<uintptr_t>(c.out) % (4 * sizeof(T)) == 0;
   auto kernel = slice_kernel<F4, BN, T, XT>;
   static std::atomic<bool> allowed[kMaxDevices];
   rc = allow_smem(kernel, allowed, current_device(), C::kSmem);
@@ -916,14 +993,25 @@ int launch_slice(const Call& c) {
   return ko::check_launch(who);
 }
 
+// Which kernel, by the numbers of 256 x 128 tiles and of pipeline stages along K (bf16 outputs, us on B200):
+//   up to 64 rows, the slices: 48 x 8192 x 8192 in 10.1 against 15.3 with pairs.
+//   More rows and fewer tiles than stages, the slices too, for the pairs would leave most SMs idle behind a long K:
+//   300 x 4096 x 512 in 8.0 against 9.9; with more tiles, the pairs: 1200 x 4096 x 512 in 10.0 against 10.6 and
+//   1200 x 1024 x 1024 in 6.6 against 8.4. One tile of 128 rows reads the weight once, and the slices keep a long K
+//   longer: 128 x 8192 x 8192 in 13.1 against 15.9.
+//   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.7 against 11.6) or K is at
+//   most two stages, where the epilogue counts (25664 x 384 x 1536 in 24.1 against 29.5); else 256 x 256, with less to
+//   load for a product (25664 x 1024 x 1536 in 29.3 against 34.4, 8192 x 4096 x 8192 in 111 against 149).
 template <bool F4, typename T>
 int launch(const Call& c) {
-  const int64_t pair_tiles = ((c.M + 255) / 256) * ((c.N + 255) / 256);
-  if (c.M > 128 && pair_tiles >= 24) return launch_pair<F4, T>(c);
+  const int64_t tiles = ((c.M + 255) / 256) * ((c.N + 127) / 128);
+  const int64_t stages = (c.Kp + Elem<F4>::kStageK - 1) / Elem<F4>::kStageK;
   if (c.M <= 16) return launch_slice<F4, 16, T>(c);
   if (c.M <= 32) return launch_slice<F4, 32, T>(c);
   if (c.M <= 64) return launch_slice<F4, 64, T>(c);
-  return launch_slice<F4, 128, T>(c);
+  if (tiles <= stages || (c.M <= 128 && stages >= 32)) return launch_slice<F4, 128, T>(c);
+  if (tiles <= c.info->sm_count / 2 || stages <= 2) return launch_pair<F4, 128, T>(c);
+  return launch_pair<F4, 256, T>(c);
 }
 
 template <typename T>

