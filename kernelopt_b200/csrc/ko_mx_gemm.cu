@@ -199,14 +199,17 @@ constexpr int kPairThreads = 18 * 32;
 
 template <bool F4, int BN>
 struct PairCfg {
-  static constexpr int kStages = BN == 256 ? 4 : 6;  // what fits beside the staging tiles
+  // Rows of the staging tiles: 128 bytes, or 64 where the room is better used for a stage more (BN 256: 8192 x 4096 x 8192
+  // in mxfp8 in 185 us with five stages, in 193 with four and 128-byte rows).
+  static constexpr int kRow = BN == 256 ? 64 : 128;
+  static constexpr int kStages = BN == 256 ? 5 : 6;
   static constexpr uint32_t kA = 128 * 128, kW = BN / 2 * 128;
   static constexpr uint32_t kSfa = 512 * Elem<F4>::kKt, kSfw = BN / 128 * kSfa;
   static constexpr uint32_t kOffSf = kA + kW;
   static constexpr uint32_t kStage = (kOffSf + kSfa + kSfw + 1023) / 1024 * 1024;
   static constexpr uint32_t kTx = 2 * (kA + Elem<F4>::kTxW * BN / 256 + kSfa + kSfw);  // both CTAs
   static constexpr uint32_t kOffStaging = kStages * kStage;
-  static constexpr uint32_t kStaging = 32 * 128;  // 32 rows of 128 bytes for each epilogue warp
+  static constexpr uint32_t kStaging = 32 * kRow;  // 32 rows for each epilogue warp
   static constexpr uint32_t kOffBias = kOffStaging + 16 * kStaging;  // 64 columns for each epilogue warp
   static constexpr uint32_t kOffBars = kOffBias + 16 * 64 * 4;
   static constexpr uint32_t kSmem = 1024 + kOffBars + 256;
@@ -376,7 +379,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     float* bias = reinterpret_cast<float*>(smem + C::kOffBias) + e * 64;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const uint32_t free_bars = cluster_map(smem_addr(acc_free), 0);
-    constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a staging row
+    constexpr int kCols = C::kRow / static_cast<int>(sizeof(T));  // columns of a staging row: 64, 32 or 16
+    // the swizzle of 128-byte or 64-byte rows: 16-byte chunk j of row r is at chunk (j ^ swz(r))
+    auto swz = [](int r) { return C::kRow == 128 ? (r & 7) : ((r >> 1) & 3); };
     // first tensor-memory column and first row and column of the output of this warp's part of tile t (the local-th)
     auto part_of = [&](int t, int local, int& col, int& row0, int& col0) {
       int mt, nt;
@@ -433,7 +438,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (!kBoth) release();
         continue;
       }
-      constexpr bool kWide = sizeof(T) == 4;  // 32 columns fill a staging row, else all 64 do
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const uint32_t(&rc)[32] = r[kBoth ? c : 0];
@@ -452,43 +456,48 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           v[4 * j + 3] = __uint_as_float(rc[4 * j + 3]) + b.w;
         }
         apply_act(v, a.act);
-        if (kWide || c == 0) {
-          if (lane == 0) bulk_wait_read<0>();  // the last store has left the tile
-          __syncwarp();
-        }
-        if constexpr (kWide) {
+        constexpr int kPart = kCols < 32 ? kCols : 32;  // columns of this chunk in one store
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(stg + lane * 128 + (((c * 4 + j) ^ (lane & 7)) << 4)) =
-                make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
-                           pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7]));
-          if (c == 0) continue;
-        }
-        const int pc = c0 + (kWide ? c * 32 : 0);
-        if (a.tma_out) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0 && pc < a.N) {
-            tma_store_2d(&map_out, stg, pc, r0);
-            bulk_commit();
+        for (int part = 0; part < 32 / kPart; ++part) {
+          const float* w = v + part * kPart;
+          if (kCols <= 32 || c == 0) {
+            if (lane == 0) bulk_wait_read<0>();  // the last store has left the tile
+            __syncwarp();
           }
-        } else {
-          __syncwarp();
-          T* out = static_cast<T*>(a.out);
-          const int rows = static_cast<int>(min(int64_t(32), a.M - r0));
-          for (int rr = 0; rr < rows; ++rr)
-            for (int c = lane; c < kCols; c += 32)
-              if (pc + c < a.N) {
-                const int byte = c * static_cast<int>(sizeof(T));
-                out[static_cast<int64_t>(r0 + rr) * a.N + pc + c] =
-                    *reinterpret_cast<const T*>(stg + rr * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
-              }
-          __syncwarp();
+          constexpr int kChunks = kPart * static_cast<int>(sizeof(T)) / 16;
+          const int first = kCols <= 32 ? 0 : c * kChunks;
+#pragma unroll
+          for (int j = 0; j < kChunks; ++j) {
+            uint4 u;
+            if constexpr (sizeof(T) == 4)
+              u = make_uint4(__float_as_uint(w[4 * j]), __float_as_uint(w[4 * j + 1]), __float_as_uint(w[4 * j + 2]),
+                             __float_as_uint(w[4 * j + 3]));
+            else
+              u = make_uint4(pack2<T>(w[8 * j], w[8 * j + 1]), pack2<T>(w[8 * j + 2], w[8 * j + 3]),
+                             pack2<T>(w[8 * j + 4], w[8 * j + 5]), pack2<T>(w[8 * j + 6], w[8 * j + 7]));
+            *reinterpret_cast<uint4*>(stg + lane * C::kRow + (((first + j) ^ swz(lane)) << 4)) = u;
+          }
+          if (kCols > 32 && c == 0) continue;  // the other chunk fills the row
+          const int pc = c0 + (kCols > 32 ? 0 : c * 32 + part * kPart);
+          if (a.tma_out) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && pc < a.N) {
+              tma_store_2d(&map_out, stg, pc, r0);
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            T* out = static_cast<T*>(a.out);
+            const int rows = static_cast<int>(min(int64_t(32), a.M - r0));
+            for (int i = lane; i < rows * kCols; i += 32) {
+              const int rr = i / kCols, cc = i % kCols, byte = cc * static_cast<int>(sizeof(T));
+              if (pc + cc < a.N)
+                out[static_cast<int64_t>(r0 + rr) * a.N + pc + cc] =
+                    *reinterpret_cast<const T*>(stg + rr * C::kRow + (((byte >> 4) ^ swz(rr)) << 4) + (byte & 15));
+            }
+            __syncwarp();
+          }
         }
       }
     }
@@ -907,7 +916,8 @@ int launch_pair(const Call& c) {
   mo = ma;  // not used without tma_out
   if (!rc && tma_out)
     rc = encode_2d(&mo, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, c.out, c.N, c.M,
-                   c.N * es, static_cast<uint32_t>(128 / es), 32, CU_TENSOR_MAP_SWIZZLE_128B, who);
+                   c.N * es, static_cast<uint32_t>(C::kRow / es), 32,
+                   C::kRow == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, who);
   if (rc) return rc;
   PairArgs a{};
   a.bias = c.bias;
