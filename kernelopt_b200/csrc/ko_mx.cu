@@ -1,9 +1,7 @@
 // Microscaled quantisation, its inverse, the 4-bit weight layout, and the residual + root-mean-square norm whose output
 // can be microscaled in the same pass. Formats and layout: ko_mx.cuh.
 //
-// All of these read and write each byte once; HBM bounds them where the instructions per element are kept few. Eight
-// consecutive elements belong to a lane, four lanes to a block of 32 and sixteen lanes to the 128 elements of a scale
-// word, so a block's largest magnitude is two shuffles and its four scales are written as one 32-bit word.
+// All of these read and write each byte once; HBM bounds them where the instructions per element are kept few.
 #include <cmath>
 #include <string>
 
@@ -16,70 +14,67 @@ using namespace komx;
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------------------------------------
-// Quantisation and its inverse: half a warp takes the 128 elements of a scale word of kRows neighbouring rows, all loads
-// before the arithmetic. Items run over k tiles, then row groups; the rows that fill the last tile of 128 are included in
-// quantisation (scale words 0, no codes).
+// Quantisation: L lanes take a block of 32 elements. L 1 for 16-bit rows that are whole groups of eight: a block's scale is
+// worked out once and without shuffles (8192 x 8192 bf16 in 26.8 us, 6.3 TB/s; with four lanes to a block 115 instructions
+// for eight elements, bound by their issue, 36.7 us). L 2 for such fp32 rows, 64 bytes to a lane (25600 x 1536 in 26.7 us,
+// 6.7 TB/s; 30.2 with L 1 or 4). L 4 for rows that are read element by element, from nearer addresses (1203 x 1001 in
+// 2.7 us, 6.1 with L 1). Items run over the blocks of a row, then rows; the rows that fill the last tile of 128 are
+// included (scale 0, no codes).
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kRows = 4;
-
-struct Item {
-  int64_t row;
-  uint32_t kt;
-  int lane16;
-};
-__device__ __forceinline__ bool item_of(int64_t items, uint32_t ktiles, Item& it) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
-  if (item >= items) return false;
-  const int64_t group = items <= 0xffffffffll ? static_cast<uint32_t>(item) / ktiles : item / ktiles;
-  it.row = group * kRows;
-  it.kt = static_cast<uint32_t>(item - group * ktiles);
-  it.lane16 = threadIdx.x & 15;
-  return true;
-}
-
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT, bool VEC, int L>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t K,
-                                                            int64_t ldx, int64_t items, uint32_t ktiles,
+                                                            int64_t ldx, int64_t items, uint32_t kblocks,
                                                             int64_t code_pitch, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales) {
-  Item it;
-  if (!item_of(items, ktiles, it)) return;
-  uint8_t* word = scales + scale_word_offset(it.row, it.kt, ktiles);  // the group's rows are 16 bytes apart
-  const int real = static_cast<int>(min(int64_t(kRows), rows - it.row));
-  const int64_t k = static_cast<int64_t>(it.kt) * 128 + it.lane16 * 8;
-  const int left = static_cast<int>(K - k);
-  const T* p = x + it.row * ldx + k;
-  uint8_t* code = codes + it.row * code_pitch + static_cast<int64_t>(it.kt) * (FMT == KO_MXFP4 ? 64 : 128) +
-                  it.lane16 * (FMT == KO_MXFP4 ? 4 : 8);
-  Raw8<T> r[kRows];
+  // items: a multiple of 512 blocks, so every warp is whole, in range or not, and the lanes of a block stay together
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
+  if (item >= items) return;
+  const int part = threadIdx.x % L;
+  const int64_t row = items <= 0xffffffffll ? static_cast<uint32_t>(item) / kblocks : item / kblocks;
+  const uint32_t kb = static_cast<uint32_t>(item - row * kblocks);
+  uint8_t* scale = scales + scale_word_offset(row, kb >> 2, kblocks >> 2) + (kb & 3);
+  const bool real = row < rows;
+  constexpr int kWords = (FMT == KO_MXFP4 ? 4 : 8) / L;
+  uint32_t c[kWords];
+  const int64_t k = static_cast<int64_t>(kb) * 32 + part * (32 / L);
+  const uint32_t byte =
+      quantize_block<T, FMT, VEC, L>(x + (real ? row : 0) * ldx + k, real ? static_cast<int>(K - k) : 0, c);
+  if (part == 0) *scale = static_cast<uint8_t>(byte);  // 0 for a row of the fill
+  if (!real) return;
+  uint8_t* dst = codes + row * code_pitch + static_cast<int64_t>(kb) * (kWords * L * 4) + part * (kWords * 4);
+  if constexpr (kWords == 1) *reinterpret_cast<uint32_t*>(dst) = c[0];
+  else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
+  else {
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) r[i] = load8<T, VEC>(p + i * ldx, i < real ? left : 0);
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    if (i < real) {
-      float v[8];
-      widen8(r[i], v);
-      quantize_group<FMT>(v, amax_bits8(r[i]), 0xffffu << (threadIdx.x & 16), code + i * code_pitch, word + 16 * i);
-    } else if (it.lane16 == 0) {
-      *reinterpret_cast<uint32_t*>(word + 16 * i) = 0u;
-    }
+    for (int i = 0; i < kWords; i += 4)
+      *reinterpret_cast<uint4*>(dst + 4 * i) = make_uint4(c[i], c[i + 1], c[i + 2], c[i + 3]);
   }
 }
+
+// ---------------------------------------------------------------------------------------------------------
+// The inverse: half a warp takes the 128 elements of a scale word of kRows neighbouring rows, all loads before the
+// arithmetic, and a lane eight elements of each, which it stores at once.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int kRows = 4;
 
 template <typename T, int FMT, bool VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, int64_t rows,
                                                               int64_t K, int64_t items, uint32_t ktiles,
                                                               int64_t code_pitch, T* __restrict__ out) {
-  Item it;
-  if (!item_of(items, ktiles, it)) return;
-  const uint8_t* word = scales + scale_word_offset(it.row, it.kt, ktiles) + (it.lane16 >> 2);
-  const int real = static_cast<int>(min(int64_t(kRows), rows - it.row));
-  const int64_t k = static_cast<int64_t>(it.kt) * 128 + it.lane16 * 8;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
+  if (item >= items) return;
+  const int64_t group = items <= 0xffffffffll ? static_cast<uint32_t>(item) / ktiles : item / ktiles;
+  const int64_t row = group * kRows;
+  const uint32_t kt = static_cast<uint32_t>(item - group * ktiles);
+  const int lane16 = threadIdx.x & 15;
+  const uint8_t* word = scales + scale_word_offset(row, kt, ktiles) + (lane16 >> 2);  // the group's rows: 16 bytes apart
+  const int real = static_cast<int>(min(int64_t(kRows), rows - row));
+  const int64_t k = static_cast<int64_t>(kt) * 128 + lane16 * 8;
   const int left = static_cast<int>(K - k);
-  const uint8_t* code = codes + it.row * code_pitch + static_cast<int64_t>(it.kt) * (FMT == KO_MXFP4 ? 64 : 128) +
-                        it.lane16 * (FMT == KO_MXFP4 ? 4 : 8);
-  T* dst = out + it.row * K + k;
+  const uint8_t* code = codes + row * code_pitch + static_cast<int64_t>(kt) * (FMT == KO_MXFP4 ? 64 : 128) +
+                        lane16 * (FMT == KO_MXFP4 ? 4 : 8);
+  T* dst = out + row * K + k;
   uint2 c[kRows];
   uint32_t byte[kRows];
 #pragma unroll
@@ -155,7 +150,8 @@ __global__ void __launch_bounds__(kThreads) pack_weight_kernel(const T* __restri
 // ---------------------------------------------------------------------------------------------------------
 // Residual + root-mean-square norm. T threads share a row and keep its NV groups of eight elements each in fp32
 // registers from the load to the store, so h and o are read once; the sum of squares is a shuffle tree and, for rows of
-// more than a warp, one exchange through shared memory, both in a fixed order. OUT: -1 writes y in the input's type, else
+// more than a warp, one exchange through shared memory, both in a fixed order. Four lanes hold a block of 32 and sixteen
+// the 128 elements of a scale word, so a quantised block costs two shuffles and its scales are stored a word at a time. OUT: -1 writes y in the input's type, else
 // the MX format.
 // ---------------------------------------------------------------------------------------------------------
 struct NormArgs {
@@ -312,19 +308,18 @@ int dispatch_norm(const NormArgs& a, int out, bool vec, cudaStream_t s) {
 template <typename T, int FMT>
 int launch_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, void* codes, void* scales, bool vec,
                     cudaStream_t s) {
-  const int64_t ktiles = padded_k(K) / 128, items = (rows + 127) / 128 * (128 / kRows) * ktiles;
-  const int64_t blocks = (items + kThreads / 16 - 1) / (kThreads / 16);
-  if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_quantize_mx: too many elements");
-  const int64_t pitch = code_pitch(K, FMT);
-  uint8_t *c = static_cast<uint8_t*>(codes), *sc = static_cast<uint8_t*>(scales);
-  const unsigned g = static_cast<unsigned>(blocks);
-  if (vec)
-    quantize_kernel<T, FMT, true><<<g, kThreads, 0, s>>>(static_cast<const T*>(x), rows, K, ldx, items,
-                                                         static_cast<uint32_t>(ktiles), pitch, c, sc);
-  else
-    quantize_kernel<T, FMT, false><<<g, kThreads, 0, s>>>(static_cast<const T*>(x), rows, K, ldx, items,
-                                                          static_cast<uint32_t>(ktiles), pitch, c, sc);
-  return ko::check_launch("ko_quantize_mx");
+  const int64_t kblocks = padded_k(K) / 32, items = (rows + 127) / 128 * 128 * kblocks;
+  auto go = [&](auto kernel, int lanes) {
+    const int64_t blocks = (items * lanes + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_quantize_mx: too many elements");
+    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(
+        static_cast<const T*>(x), rows, K, ldx, items, static_cast<uint32_t>(kblocks), code_pitch(K, FMT),
+        static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
+    return ko::check_launch("ko_quantize_mx");
+  };
+  if (!vec) return go(quantize_kernel<T, FMT, false, 4>, 4);
+  constexpr int L = sizeof(T) == 2 ? 1 : 2;
+  return go(quantize_kernel<T, FMT, true, L>, L);
 }
 
 template <typename T>

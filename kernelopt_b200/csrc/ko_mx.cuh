@@ -239,6 +239,42 @@ __device__ __forceinline__ int64_t scale_word_offset(int64_t row, int64_t ktile,
   return ((row >> 7) * ktiles + ktile) * 512 + (r & 31) * 16 + (r >> 5) * 4;
 }
 
+// 32 / L elements of a block at `p`, of which `left` (any integer) lie before the end of the row and the others are zero,
+// the block being shared by L neighbouring lanes that call this together: the lane's codes (16 / L bytes in mxfp4, 32 / L in
+// mxfp8) and the block's scale byte.
+template <typename T, int FMT, bool VEC, int L>
+__device__ __forceinline__ uint32_t quantize_block(const T* p, int left, uint32_t (&code)[(FMT == KO_MXFP4 ? 4 : 8) / L]) {
+  constexpr int G = 4 / L;  // groups of eight
+  Raw8<T> r[G];
+  uint32_t m = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) r[g] = load8<T, VEC>(p + g * 8, left - g * 8);
+#pragma unroll
+  for (int g = 0; g < G; ++g) m = max(m, amax_bits8(r[g]));
+#pragma unroll
+  for (int s = 1; s < L; s <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
+  const uint32_t byte = scale_byte<FMT>(m);
+  const float inv = scale_inverse(byte);
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    float v[8];
+    widen8(r[g], v);
+    if constexpr (FMT == KO_MXFP4) {
+      code[g] = pack_e2m1x8(v, inv);
+    } else {
+      const uint2 c = pack_e4m3x8(v, inv);
+      code[2 * g] = c.x;
+      code[2 * g + 1] = c.y;
+    }
+  }
+  // a NaN or an infinity times the zero inverse is NaN, which would convert to the largest code: such blocks are cleared
+  if (byte == 255u) {
+#pragma unroll
+    for (int i = 0; i < (FMT == KO_MXFP4 ? 1 : 2) * G; ++i) code[i] = 0u;
+  }
+  return byte;
+}
+
 // Writes the codes of a lane's eight values and, from one lane in sixteen, the scale word of their 128 elements. A group
 // of sixteen lanes that calls this together holds one row's elements [128 kt, 128 kt + 128) in order; `mask` names them, m
 // is the largest magnitude of the lane's own values, `code` the address of their codes.
@@ -250,7 +286,6 @@ __device__ __forceinline__ void quantize_group(const float (&v)[8], uint32_t m, 
   m = max(m, __shfl_xor_sync(mask, m, 2));
   const uint32_t byte = scale_byte<FMT>(m);
   const float inv = scale_inverse(byte);
-  // a NaN or an infinity times the zero inverse is NaN, which would convert to the largest code: such blocks are cleared
   if constexpr (FMT == KO_MXFP4) {
     const uint32_t c = pack_e2m1x8(v, inv);
     *reinterpret_cast<uint32_t*>(code) = byte == 255u ? 0u : c;

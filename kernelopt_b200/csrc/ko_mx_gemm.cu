@@ -490,6 +490,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             __syncwarp();
             T* out = static_cast<T*>(a.out);
             const int rows = static_cast<int>(min(int64_t(32), a.M - r0));
+#pragma unroll 8
             for (int i = lane; i < rows * kCols; i += 32) {
               const int rr = i / kCols, cc = i % kCols, byte = cc * static_cast<int>(sizeof(T));
               if (pc + cc < a.N)
@@ -554,28 +555,6 @@ struct SliceArgs {
   int64_t K, ldx;
   int x_vec;      // rows of x are whole groups of eight (groups_of_8)
 };
-
-// A block of 32 elements from k on, zero beyond K: its mxfp4 codes and its scale byte.
-template <typename XT>
-__device__ __forceinline__ uint4 quantize_block(const XT* row, int64_t k, int64_t K, bool vec, uint32_t& byte) {
-  Raw8<XT> r[4];
-  uint32_t m = 0;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int left = static_cast<int>(K - k) - g * 8;
-    r[g] = vec ? load8<XT, true>(row + k + g * 8, left) : load8<XT, false>(row + k + g * 8, left);
-  }
-  float v[4][8];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    m = max(m, amax_bits8(r[g]));
-    widen8(r[g], v[g]);
-  }
-  byte = scale_byte<KO_MXFP4>(m);
-  if (byte == 255u) return make_uint4(0u, 0u, 0u, 0u);
-  const float inv = scale_inverse(byte);
-  return make_uint4(pack_e2m1x8(v[0], inv), pack_e2m1x8(v[1], inv), pack_e2m1x8(v[2], inv), pack_e2m1x8(v[3], inv));
-}
 
 // Adds the S partial sums of rows rank, rank + S, ... of a tile and stores them. A warp takes 8 / S rows at a time and a lane
 // four columns of them: eight 128-bit reads through distributed shared memory on their way at once, added in rank order.
@@ -751,8 +730,14 @@ __global__ void __launch_bounds__(kSliceThreads)
         code[i] = make_uint4(0u, 0u, 0u, 0u);
         byte[i] = 0u;
         const int64_t k = static_cast<int64_t>(ks) * E::kStageK + b * 32;
-        if (r + 8 * i < cols && k < a.K)
-          code[i] = quantize_block(static_cast<const XT*>(a.x) + (r + 8 * i) * a.ldx, k, a.K, a.x_vec != 0, byte[i]);
+        if (r + 8 * i < cols && k < a.K) {
+          const XT* p = static_cast<const XT*>(a.x) + (r + 8 * i) * a.ldx + k;
+          const int left = static_cast<int>(a.K - k);
+          uint32_t c[4];
+          byte[i] = a.x_vec ? quantize_block<XT, KO_MXFP4, true, 1>(p, left, c)
+                            : quantize_block<XT, KO_MXFP4, false, 1>(p, left, c);
+          code[i] = make_uint4(c[0], c[1], c[2], c[3]);
+        }
       }
       if (!mbar_wait_warp(&empty[st], phase ^ 1u, abort_flag)) break;
       uint8_t* s = smem + st * C::kStage;
