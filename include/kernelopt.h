@@ -344,13 +344,16 @@ int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_fmt, const 
                     const float* bias, int64_t M, int64_t K, int64_t N, int act, void* out, int out_dtype,
                     int* dev_status, ko_stream_t stream);
 
-/* The same for a few rows that are not quantised yet: x [M][K] of x_dtype, row r at x + r * ldx elements, is quantised to
- * KO_MXFP4 inside the product's kernel, with the result of ko_quantize_mx and ko_linear_mxfp4 bit for bit. For the tokens
- * of a decoding step, where a launch of its own and the round trip through memory cost more than the quantisation. */
+/* The same for rows that are not quantised yet: x [M][K] of x_dtype, row r at x + r * ldx elements, is quantised to
+ * KO_MXFP4 and multiplied, with the result of ko_quantize_mx and ko_linear_mxfp4 bit for bit. Up to KO_MXFP4_FUSED_ROWS
+ * rows, the tokens of a decoding step, are quantised inside the product's kernel: a launch of their own and the round trip
+ * through memory would cost more, and `workspace` may be NULL. More rows go through `workspace`: 16-byte aligned,
+ * ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes (0 up to KO_MXFP4_FUSED_ROWS rows, -1 for a bad size). */
 #define KO_MXFP4_FUSED_ROWS 16
+int64_t ko_linear_quantize_mxfp4_workspace_bytes(int64_t M, int64_t K);
 int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx, const void* w_codes, const void* w_scales,
                              const float* bias, int64_t M, int64_t K, int64_t N, int act, void* out, int out_dtype,
-                             int* dev_status, ko_stream_t stream);
+                             void* workspace, int64_t workspace_bytes, int* dev_status, ko_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -68,7 +68,9 @@ SIGNATURES = {
     "ko_pack_weight_mxfp4": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp]),
     "ko_residual_rmsnorm": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _f32, _i64, _i64, _vp, _vp, _i32, _vp,
                                    _vp, _vp]),
-    "ko_linear_quantize_mxfp4": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _vp]),
+    "ko_linear_quantize_mxfp4_workspace_bytes": (_i64, [_i64, _i64]),
+    "ko_linear_quantize_mxfp4": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _i64,
+                                        _vp, _vp]),
     "ko_linear_mxfp4": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _vp]),
 }
 
@@ -109,7 +111,7 @@ LAUNCHING = {"ko_preprocess": 1, "ko_preprocess_batch": 1, "ko_residual_layernor
              "ko_wait_probe": 1, "ko_window_merge_ln": 1, "ko_window_partition_ln": 1, "ko_deform_prep": 1,
              "ko_linear_add_f32_packed": 1, "ko_sine_embed": 1, "ko_linear_small_f32": 1, "ko_box_head_f32": 1,
              "ko_quantize_mx": 1, "ko_dequantize_mx": 1, "ko_pack_weight_mxfp4": 1, "ko_residual_rmsnorm": 1,
-             "ko_linear_mxfp4": 1, "ko_linear_quantize_mxfp4": 1}
+             "ko_linear_mxfp4": 1, "ko_linear_quantize_mxfp4": 1}  # one more for rows over KO_MXFP4_FUSED_ROWS
 launch_count: dict[str, int] = {}
 
 

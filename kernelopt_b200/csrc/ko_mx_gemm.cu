@@ -1056,19 +1056,35 @@ extern "C" int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_
   return f4 ? launch<true, __half>(c) : launch<false, __half>(c);
 }
 
+extern "C" int64_t ko_linear_quantize_mxfp4_workspace_bytes(int64_t M, int64_t K) {
+  const int64_t codes = ko_mx_codes_bytes(M, K, KO_MXFP4), scales = ko_mx_scales_bytes(M, K);
+  if (codes < 0 || scales < 0) return -1;
+  return M <= kFuseRows ? 0 : (codes + 15) / 16 * 16 + scales;
+}
+
 extern "C" int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx, const void* w_codes,
                                         const void* w_scales, const float* bias, int64_t M, int64_t K, int64_t N,
-                                        int act, void* out, int out_dtype, int* dev_status, ko_stream_t stream) {
+                                        int act, void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
+                                        int* dev_status, ko_stream_t stream) {
   const char* name = "ko_linear_quantize_mxfp4";
   int rc = check_linear(name, M, K, N, act, w_codes, w_scales, bias, out, out_dtype);
   if (rc) return rc;
   auto bad = [&](const char* what) { return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
   if (!dtype_ok(x_dtype)) return bad("unknown element type");
-  if (M > kFuseRows) return bad("at most KO_MXFP4_FUSED_ROWS rows; more are quantised by ko_quantize_mx first");
   if (ldx < K) return bad("ldx must be at least K");
   if (M == 0) return KO_OK;
   if (!x || reinterpret_cast<uintptr_t>(x) % static_cast<uintptr_t>(dtype_size(x_dtype)) != 0)
     return bad("x must be given, aligned to its elements");
+  if (M > kFuseRows) {
+    if (!workspace || !ko::aligned16(workspace) || workspace_bytes < ko_linear_quantize_mxfp4_workspace_bytes(M, K))
+      return bad("the workspace must be 16-byte aligned and hold ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes");
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    uint8_t* scales = codes + (ko_mx_codes_bytes(M, K, KO_MXFP4) + 15) / 16 * 16;
+    rc = ko_quantize_mx(x, x_dtype, M, K, ldx, KO_MXFP4, codes, scales, stream);
+    if (rc) return rc;
+    return ko_linear_mxfp4(codes, scales, KO_MXFP4, w_codes, w_scales, bias, M, K, N, act, out, out_dtype, dev_status,
+                           stream);
+  }
   Call c{nullptr, nullptr, w_codes, w_scales, bias, M, K, N, padded_k(K), act, out, dev_status,
          reinterpret_cast<cudaStream_t>(stream), nullptr, x, ldx};
   rc = ko::device_or_fail(&c.info, name);

@@ -772,10 +772,14 @@ def linear_mxfp4(x, pw: PackedWeightMX, act=None, out_dtype=None, out=None):
     elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.device != dev
           or not out.is_contiguous() or out.dtype not in MX_DTYPES or out_dtype not in (None, out.dtype)):
         raise ValueError(f"out must be a contiguous {list(shape)} tensor on {dev}, float32, bfloat16 or float16")
-    tail = (*pw.ptrs, rows, pw.k, pw.n, ACTS[act], out.data_ptr(), MX_DTYPES[out.dtype], pw.status)
-    if not quantized and rows <= _lib.KO_MXFP4_FUSED_ROWS:
-        _call_on(dev, "ko_linear_quantize_mxfp4", x.data_ptr(), MX_DTYPES[x.dtype], pitch, *tail)
-    else:
-        q = x if quantized else quantize_mx(x)
-        _call_on(dev, "ko_linear_mxfp4", *q._ptrs(), MX_FORMATS[q.fmt], *tail)
+    args = (*pw.ptrs, rows, pw.k, pw.n, ACTS[act], out.data_ptr(), MX_DTYPES[out.dtype])
+    if quantized:
+        _call_on(dev, "ko_linear_mxfp4", *x._ptrs(), MX_FORMATS[x.fmt], *args, pw.status)
+        return out
+    work, size = None, 0
+    if rows > _lib.KO_MXFP4_FUSED_ROWS:  # x in mxfp4, in one buffer
+        size = _lib.lib().ko_linear_quantize_mxfp4_workspace_bytes(rows, pw.k)
+        work = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=dev)
+        _lib.launch_count["ko_linear_quantize_mxfp4"] = _lib.launch_count.get("ko_linear_quantize_mxfp4", 0) + 1
+    _call_on(dev, "ko_linear_quantize_mxfp4", x.data_ptr(), MX_DTYPES[x.dtype], pitch, *args, _ptr(work), size, pw.status)
     return out

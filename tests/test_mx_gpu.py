@@ -465,5 +465,6 @@ def test_launch_counts(cuda):
     K.linear_mxfp4(x, pw)
     K.rmsnorm(x, torch.ones(64, device=cuda), 1e-6, quantize="mxfp8").dequantize()
     K.linear_mxfp4(x.repeat(5, 1), pw)
-    assert _lib.launch_count == {"ko_pack_weight_mxfp4": 1, "ko_linear_quantize_mxfp4": 1, "ko_residual_rmsnorm": 1,
+    K.linear_mxfp4(K.quantize_mx(x), pw)
+    assert _lib.launch_count == {"ko_pack_weight_mxfp4": 1, "ko_linear_quantize_mxfp4": 3, "ko_residual_rmsnorm": 1,
                                  "ko_dequantize_mx": 1, "ko_quantize_mx": 1, "ko_linear_mxfp4": 1}

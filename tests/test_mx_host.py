@@ -55,12 +55,14 @@ A = 4096  # a stand-in for an aligned device pointer: every call below is refuse
     ("ko_linear_mxfp4", (A, A, 0, A, A, A + 2, 4, 64, 64, 0, A, 0, None, None)),   # bias unaligned
     ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 64, 64, 0, A + 1, 1, None, None)),  # out unaligned
     ("ko_linear_mxfp4", (A, A, 0, A + 16, A, None, 4, 64, 64, 0, A, 0, None, None)),  # weight codes not on 32 bytes
-    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 17, 64, 64, 0, A, 0, None, None)),   # too many rows
-    ("ko_linear_quantize_mxfp4", (A, 0, 63, A, A, None, 4, 64, 64, 0, A, 0, None, None)),    # pitch below the width
-    ("ko_linear_quantize_mxfp4", (A, 5, 64, A, A, None, 4, 64, 64, 0, A, 0, None, None)),    # unknown element type
-    ("ko_linear_quantize_mxfp4", (None, 0, 64, A, A, None, 4, 64, 64, 0, A, 0, None, None)),  # no x
-    ("ko_linear_quantize_mxfp4", (A + 1, 1, 64, A, A, None, 4, 64, 64, 0, A, 0, None, None)),  # x unaligned
-    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 4, 64, 64, 9, A, 0, None, None)),    # unknown act
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 17, 64, 64, 0, A, 0, None, 0, None, None)),  # no workspace
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 17, 64, 64, 0, A, 0, A, 1599, None, None)),  # too small
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 17, 64, 64, 0, A, 0, A + 8, 9999, None, None)),  # unaligned
+    ("ko_linear_quantize_mxfp4", (A, 0, 63, A, A, None, 4, 64, 64, 0, A, 0, None, 0, None, None)),   # pitch < width
+    ("ko_linear_quantize_mxfp4", (A, 5, 64, A, A, None, 4, 64, 64, 0, A, 0, None, 0, None, None)),   # element type
+    ("ko_linear_quantize_mxfp4", (None, 0, 64, A, A, None, 4, 64, 64, 0, A, 0, None, 0, None, None)),  # no x
+    ("ko_linear_quantize_mxfp4", (A + 1, 1, 64, A, A, None, 4, 64, 64, 0, A, 0, None, 0, None, None)),  # x unaligned
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 4, 64, 64, 9, A, 0, None, 0, None, None)),   # unknown act
 ])
 def test_bad_arguments_are_refused_on_the_host(name, args):
     with pytest.raises(ValueError, match=name):
@@ -83,6 +85,9 @@ def test_sizes():
     assert lib.ko_mx_codes_bytes(3, 129, _lib.KO_MXFP8) == 3 * 256
     assert lib.ko_mx_scales_bytes(129, 129) == 256 * 8
     assert lib.ko_mx_codes_bytes(3, 0, 0) == lib.ko_mx_codes_bytes(-1, 8, 0) == lib.ko_mx_codes_bytes(3, 8, 2) == -1
+    assert lib.ko_linear_quantize_mxfp4_workspace_bytes(16, 64) == 0
+    assert lib.ko_linear_quantize_mxfp4_workspace_bytes(17, 64) == 17 * 64 + 128 * 4 == 1600
+    assert lib.ko_linear_quantize_mxfp4_workspace_bytes(17, 0) == -1
     assert lib.ko_mx_scales_bytes(-1, 8) == lib.ko_mx_scales_bytes(1, 0) == -1
 
 
