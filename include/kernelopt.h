@@ -329,7 +329,7 @@ int ko_pack_weight_mxfp4(const void* w, int dtype, int64_t K, int64_t N, void* c
 /* v = h + (o + bias) * scale;  y = v / sqrt(mean(v^2) + eps) * gamma over rows of C (statistics and y in fp32 from the
  * unrounded v). h, o: [rows][C] of `dtype`, rows ldh / ldo elements apart; bias, scale, gamma: [C] of `dtype`; o NULL
  * = no residual (bias and scale then unused), bias / scale NULL = 0 / 1. h_out: [rows][C] receives v rounded to
- * `dtype`, or NULL; it may be h itself when ldh == C. Exactly one form of y: y [rows][C] of `dtype`, or y NULL and
+ * `dtype`, or NULL; it may be h or o itself where that is contiguous, and overlaps them in no other way. Exactly one form of y: y [rows][C] of `dtype`, or y NULL and
  * codes, scales in `fmt`. 1 <= C <= 32768. Stands beside ko_residual_layernorm for models that normalise by the root
  * mean square. */
 int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, int64_t ldo, const void* bias, const void* scale,
@@ -348,7 +348,8 @@ int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_fmt, const 
  * KO_MXFP4 and multiplied, with the result of ko_quantize_mx and ko_linear_mxfp4 bit for bit. Up to KO_MXFP4_FUSED_ROWS
  * rows, the tokens of a decoding step, are quantised inside the product's kernel: a launch of their own and the round trip
  * through memory would cost more, and `workspace` may be NULL. More rows go through `workspace`: 16-byte aligned,
- * ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes (0 up to KO_MXFP4_FUSED_ROWS rows, -1 for a bad size). */
+ * ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes (0 up to KO_MXFP4_FUSED_ROWS rows, -1 for a bad size). out must not
+ * overlap x. */
 #define KO_MXFP4_FUSED_ROWS 16
 int64_t ko_linear_quantize_mxfp4_workspace_bytes(int64_t M, int64_t K);
 int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx, const void* w_codes, const void* w_scales,

@@ -435,8 +435,15 @@ extern "C" int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, in
   if (!h || !gamma) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
   if (!o && (bias || scale))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "bias and scale belong to o");
-  if (h_out == h && ldh != C)
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "h_out may be h only where h is contiguous");
+  // A row is read whole before it is written, by the threads that write it: in place is fine, any other overlap is not.
+  const int64_t elem = dtype_size(dtype);
+  auto meets = [&](const void* a, int64_t lda) {
+    const char *a0 = static_cast<const char*>(a), *b0 = static_cast<const char*>(h_out);
+    const bool apart = !a || !h_out || a0 + ((rows - 1) * lda + C) * elem <= b0 || b0 + rows * C * elem <= a0;
+    return !apart && !(a0 == b0 && (lda == C || rows == 1));
+  };
+  if (meets(h, ldh) || meets(o, ldo))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "h_out overlaps h or o other than in place (the same contiguous rows)");
   const int64_t es = dtype_size(dtype);
   bool vec = ldh % 8 == 0 && (!o || ldo % 8 == 0);
   const void* elems[] = {h, o, bias, scale, gamma, h_out, y};

@@ -319,10 +319,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
       }
-      if (!ok) {  // the loads in flight must land before the CTA leaves; they take microseconds
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 10000000ull) {}
-      }
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -505,6 +501,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (lane == 0) bulk_wait<0>();  // the stores have left shared memory and are written
   }
   tc_fence_before();
+  __syncthreads();
+  // After an abort loads may be in flight that no MMA waited for. They land within microseconds, and their barrier may be
+  // the peer's, so this CTA gives them ten milliseconds before it leaves.
+  if (threadIdx.x == 0 && *abort_flag) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 10000000ull) {}
+  }
   __syncthreads();
   cluster_sync();  // neither CTA leaves while the other's arrivals, copies or MMAs may still reach it
   if (warp == 1) {
@@ -1075,6 +1078,9 @@ extern "C" int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx,
   if (M == 0) return KO_OK;
   if (!x || reinterpret_cast<uintptr_t>(x) % static_cast<uintptr_t>(dtype_size(x_dtype)) != 0)
     return bad("x must be given, aligned to its elements");
+  const char *x0 = static_cast<const char*>(x), *out0 = static_cast<const char*>(out);
+  if (x0 < out0 + M * N * dtype_size(out_dtype) && out0 < x0 + ((M - 1) * ldx + K) * dtype_size(x_dtype))
+    return bad("out overlaps x");
   if (M > kFuseRows) {
     if (!workspace || !ko::aligned16(workspace) || workspace_bytes < ko_linear_quantize_mxfp4_workspace_bytes(M, K))
       return bad("the workspace must be 16-byte aligned and hold ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes");

@@ -678,7 +678,8 @@ def residual_rmsnorm(h, o, bias, scale, gamma, eps, quantize=None, h_out=None):
     """Returns (v, y) with v = h + (o + bias) * scale and y = v / sqrt(mean(v^2) + eps) * gamma over the last dimension
     (width <= 32768), both computed in fp32: residual_layernorm's arguments for a model that normalises by the root
     mean square. h and o: [..., C] float32, bfloat16 or float16 (any even row pitch); bias and scale [C] or None (0 / 1);
-    gamma [C]; all of one type. v is returned in that type, in h_out where given ([..., C] contiguous, possibly h); y
+    gamma [C]; all of one type. v is returned in that type, in h_out where given ([..., C] contiguous; h or o itself, or
+    apart from both); y
     too, or with quantize "mxfp8" / "mxfp4" as an MXTensor, quantised from fp32 in the same pass."""
     rows, ldh = _rows(h, "h")
     if o.shape != h.shape:

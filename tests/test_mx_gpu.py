@@ -76,11 +76,12 @@ def test_quantize_bit_exact(cuda, rows, k, dtype, fmt):
         assert torch.equal(v, w), f"dequantize to {out}"
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("fmt", FMTS)
-def test_quantize_every_bf16_value(cuda, fmt):
-    """All finite bfloat16 patterns, subnormals and both ends included, in blocks of 32 consecutive patterns."""
+def test_quantize_every_16_bit_value(cuda, fmt, dtype):
+    """All finite patterns, subnormals and both ends included, in blocks of 32 consecutive patterns."""
     bits = torch.arange(65536, dtype=torch.int32).to(torch.int16)
-    x = bits.view(torch.bfloat16).to(cuda)
+    x = bits.view(dtype).to(cuda)
     x = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).reshape(64, 1024)
     check_quantized(K.quantize_mx(x, fmt), np64(x))
     y = x.t().contiguous()                               # the same values beside others of every size
@@ -215,6 +216,12 @@ def test_rmsnorm_slices_in_place_and_shapes(cuda, dtype):
     mine = h.clone()
     v2, y2 = K.residual_rmsnorm(mine, o, None, None, gamma, 1e-5, h_out=mine)
     assert v2 is mine and torch.equal(v, v2) and torch.equal(y, y2) and v.shape == (4, 10, 256)
+    mine = o.clone()
+    v2, y2 = K.residual_rmsnorm(h, mine, None, None, gamma, 1e-5, h_out=mine)
+    assert torch.equal(v, v2) and torch.equal(y, y2)
+    flat = torch.zeros(12 * 256, dtype=dtype, device=cuda)
+    with pytest.raises(ValueError, match="overlaps"):
+        K.residual_rmsnorm(flat[:2560].view(10, 256), o[0], None, None, gamma, 1e-5, h_out=flat[256:2816].view(10, 256))
     assert K.rmsnorm(h[:0], gamma, 1e-5).shape == (0, 10, 256)
     assert K.rmsnorm(h[:0], gamma, 1e-5, quantize="mxfp8").shape == (0, 10, 256)
 
@@ -351,6 +358,66 @@ def test_linear_rows_do_not_meet(cuda, m, fmt):
     buf = torch.full((m + 2, n), 7.0, device=cuda)
     K.linear_mxfp4(K.quantize_mx(x, fmt), K.pack_weight_mxfp4(w, b), out=buf[1:m + 1])
     assert torch.equal(buf[1:m + 1], base) and bool((buf[0] == 7).all()) and bool((buf[m + 1] == 7).all())
+    K.check_device_status(cuda)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [3, 70, 300])
+def test_linear_output_anywhere(cuda, m, dtype):
+    """An output that starts on its own element's alignment only, with its neighbours left as they were."""
+    k, n = 320, 264
+    x = acts(m, k, 3, dtype, cuda)
+    w, b = weight(k, n, 4, dtype, cuda)
+    pw = K.pack_weight_mxfp4(w, b)
+    want = K.linear_mxfp4(x, pw, "relu")
+    flat = torch.full((m * n + 9,), 7.0, dtype=dtype, device=cuda)
+    for lead in (1, 2, 8):
+        flat.fill_(7.0)
+        K.linear_mxfp4(x, pw, "relu", out=flat[lead:lead + m * n].view(m, n))
+        assert torch.equal(flat[lead:lead + m * n].view(m, n), want)
+        assert bool((flat[:lead] == 7).all()) and bool((flat[lead + m * n:] == 7).all())
+    x0 = torch.zeros(m, 256, dtype=dtype, device=cuda)
+    with pytest.raises(ValueError, match="overlaps"):
+        K.linear_mxfp4(x0, K.pack_weight_mxfp4(w[:256, :256].contiguous()), out=x0)
+    K.check_device_status(cuda)
+
+
+def test_gelu_at_the_ends(cuda):
+    """Infinities, NaN, and values far on both sides, reached through the bias of a product of zeros."""
+    v = torch.tensor([float("inf"), -float("inf"), float("nan"), 0.0, 100.0, -100.0, 1e-30, -1e-30, 6.0, -6.0, -5.5, -9.0],
+                     device=cuda)
+    want = 0.5 * v.double() * torch.special.erfc(-v.double() / 2 ** 0.5)
+    for m in (1, 20, 100):
+        got = K.linear_mxfp4(torch.zeros(m, 64, device=cuda), K.pack_weight_mxfp4(torch.ones(64, 12, device=cuda), v), "gelu")
+        assert bool((got == got[0]).logical_or(torch.isnan(got)).all())
+        g = got[0].double()
+        assert g[0] == float("inf") and g[1] == 0 and bool(torch.isnan(g[2])) and g[3] == 0
+        # |v| q within 8e-8, and q within 3e-5 of itself up to 6; beyond that q is below 1e-9
+        assert bool(((g - want)[3:].abs() <= 1e-7 + want[3:].abs() * 2.0 ** -22).all())
+        assert bool(((g - want)[9:11].abs() <= want[9:11].abs() * 4e-5).all())
+
+
+def test_more_than_2_to_the_31_elements(cuda):
+    """The last rows of tensors whose offsets pass 32 bits, against the same rows on their own."""
+    rows, k = 70001, 32768                                     # 2.3e9 elements
+    x = torch.empty((rows, k), dtype=torch.bfloat16, device=cuda)
+    x[:-4] = 1
+    x[-4:] = acts(4, k, 5, torch.bfloat16, cuda)
+    for fmt in FMTS:
+        q, part = K.quantize_mx(x, fmt), K.quantize_mx(x[-4:], fmt)
+        assert torch.equal(q.codes[-4:].view(torch.uint8), part.codes.view(torch.uint8))
+        v = q.dequantize(torch.bfloat16)
+        assert torch.equal(v[-4:], part.dequantize(torch.bfloat16)) and bool((v[-5] == 1).all())
+        del q, v
+    gamma = torch.ones(k, dtype=torch.bfloat16, device=cuda)
+    v, y = K.residual_rmsnorm(x, x, None, None, gamma, 1e-6, quantize="mxfp8")
+    v4, y4 = K.residual_rmsnorm(x[-4:], x[-4:], None, None, gamma, 1e-6, quantize="mxfp8")
+    assert torch.equal(v[-4:], v4) and torch.equal(y.codes[-4:].view(torch.uint8), y4.codes.view(torch.uint8))
+    del v, y
+    a = acts(rows, 32, 6, torch.bfloat16, cuda)                # sums of 32 terms are exact in every form of the product
+    pw = K.pack_weight_mxfp4(weight(32, k, 7, torch.bfloat16, cuda)[0])
+    got = K.linear_mxfp4(a, pw)
+    assert torch.equal(got[-4:], K.linear_mxfp4(a[-4:], pw)) and torch.equal(got[:4], K.linear_mxfp4(a[:4], pw))
     K.check_device_status(cuda)
 
 

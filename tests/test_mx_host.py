@@ -43,6 +43,10 @@ A = 4096  # a stand-in for an aligned device pointer: every call below is refuse
     ("ko_residual_rmsnorm", (A, 64, A, 64, None, None, A, 0, 1e-6, 4, 64, A, None, 9, A, A, None)),        # format
     ("ko_residual_rmsnorm", (A, 64, None, 0, A, None, A, 0, 1e-6, 4, 64, A, A, 0, None, None, None)),      # bias, no o
     ("ko_residual_rmsnorm", (A, 72, A, 64, None, None, A, 0, 1e-6, 4, 64, A, A, 0, None, None, None)),     # h_out is a
+    ("ko_residual_rmsnorm", (A, 64, 2 * A, 64, None, None, A, 0, 1e-6, 4, 64, A + 256, 9 * A, 0, None, None, None)),  # h_out
+    ("ko_residual_rmsnorm", (9 * A, 64, A, 65, None, None, A, 0, 1e-6, 4, 64, A, 5 * A, 0, None, None, None)),  # overlaps
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 4, 64, 64, 0, A + 512, 0, None, 0, None, None)),  # out in x
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, 4, 64, 64, 0, A - 512, 0, None, 0, None, None)),  # x in out
     ("ko_residual_rmsnorm", (A, 64, A + 1, 64, None, None, A, 1, 1e-6, 4, 64, A, A, 0, None, None, None)),  # strided h
     ("ko_linear_mxfp4", (A, A, 0, A, A, None, -1, 64, 64, 0, A, 0, None, None)),   # M < 0
     ("ko_linear_mxfp4", (A, A, 0, A, A, None, 4, 0, 64, 0, A, 0, None, None)),     # K = 0
@@ -120,6 +124,31 @@ def test_row_pitch_rules():
             K._rows(bad, "t")
     with pytest.raises(ValueError):
         K._rows(t.double(), "t")
+
+
+def test_calls_go_to_the_device_of_their_tensors(monkeypatch):
+    """_call_on launches on the current stream of the tensors' device, and makes that device current for the call only
+    where it is not."""
+    seen, entered = [], []
+
+    class Guard:
+        def __init__(self, device):
+            entered.append(device)
+
+        def __enter__(self):
+            pass
+
+        def __exit__(self, *exc):
+            entered.append("left")
+
+    monkeypatch.setattr(K, "call", lambda name, *args: seen.append((name, args)))
+    monkeypatch.setattr(K, "_raw_stream", lambda index: 1000 + index)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    K._call_on(torch.device("cuda:0"), "f", 1, 2)
+    assert seen == [("f", (1, 2, 1000))] and not entered
+    K._call_on(torch.device("cuda:1"), "g", 3)
+    assert seen[1] == ("g", (3, 1001)) and entered == [torch.device("cuda:1"), "left"]
 
 
 def test_oracle_against_hand_computed_blocks():
