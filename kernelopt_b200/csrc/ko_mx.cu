@@ -37,8 +37,9 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const T* __restrict_
   constexpr int kWords = (FMT == KO_MXFP4 ? 4 : 8) / L;
   uint32_t c[kWords];
   const int64_t k = static_cast<int64_t>(kb) * 32 + part * (32 / L);
-  const uint32_t byte =
-      quantize_block<T, FMT, VEC, L>(x + (real ? row : 0) * ldx + k, real ? static_cast<int>(K - k) : 0, c);
+  Raw8<T> r[4 / L];
+  load_block<T, VEC>(x + (real ? row : 0) * ldx + k, real ? static_cast<int>(K - k) : 0, r);
+  const uint32_t byte = quantize_block<T, FMT, L>(r, c);
   if (part == 0) *scale = static_cast<uint8_t>(byte);  // 0 for a row of the fill
   if (!real) return;
   uint8_t* dst = codes + row * code_pitch + static_cast<int64_t>(kb) * (kWords * L * 4) + part * (kWords * 4);

@@ -239,16 +239,18 @@ __device__ __forceinline__ int64_t scale_word_offset(int64_t row, int64_t ktile,
   return ((row >> 7) * ktiles + ktile) * 512 + (r & 31) * 16 + (r >> 5) * 4;
 }
 
-// 32 / L elements of a block at `p`, of which `left` (any integer) lie before the end of the row and the others are zero,
-// the block being shared by L neighbouring lanes that call this together: the lane's codes (16 / L bytes in mxfp4, 32 / L in
-// mxfp8) and the block's scale byte.
-template <typename T, int FMT, bool VEC, int L>
-__device__ __forceinline__ uint32_t quantize_block(const T* p, int left, uint32_t (&code)[(FMT == KO_MXFP4 ? 4 : 8) / L]) {
-  constexpr int G = 4 / L;  // groups of eight
-  Raw8<T> r[G];
-  uint32_t m = 0;
+// 32 / L elements of a block at `p`, of which `left` (any integer) lie before the end of the row; the others are zero.
+template <typename T, bool VEC, int G>
+__device__ __forceinline__ void load_block(const T* p, int left, Raw8<T> (&r)[G]) {
 #pragma unroll
   for (int g = 0; g < G; ++g) r[g] = load8<T, VEC>(p + g * 8, left - g * 8);
+}
+// Their codes (16 / L bytes in mxfp4, 32 / L in mxfp8) and the block's scale byte, the block being shared by L neighbouring
+// lanes that call this together.
+template <typename T, int FMT, int L>
+__device__ __forceinline__ uint32_t quantize_block(const Raw8<T> (&r)[4 / L], uint32_t (&code)[(FMT == KO_MXFP4 ? 4 : 8) / L]) {
+  constexpr int G = 4 / L;  // groups of eight
+  uint32_t m = 0;
 #pragma unroll
   for (int g = 0; g < G; ++g) m = max(m, amax_bits8(r[g]));
 #pragma unroll

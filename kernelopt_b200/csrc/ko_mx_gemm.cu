@@ -522,11 +522,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // the product comes out transposed: a thread owns one output column and a warp writes 32 neighbours of a row at a time, for
 // any N. The CTAs of a cluster share a tile and take a slice of K each; their partial sums meet in shared memory and are
 // added in rank order through distributed shared memory, so results repeat bit for bit.
-// With XT other than void the rows of A come as XT values, at most kFuseRows of them, and warps 2 and 3 quantise them to
-// mxfp4 on the way into shared memory, a block of 32 to a thread: for a handful of tokens that costs less than a launch of
-// its own, and every CTA needs only its slice of them.
+// With XT other than void the rows of A come as XT values, at most kFuseRows of them, and four groups of two more warps
+// quantise them to mxfp4 on the way into shared memory, each every fourth stage and a block of 32 to a thread: for a handful
+// of tokens that costs less than a launch of its own, and every CTA needs only its slice of them. (One group, even with the
+// next stage's elements on their way, was the slowest part: 1 x 8192 x 8192 in 13.2 us, 10.8 with four.)
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kSliceThreads = 128;
+constexpr int kSliceThreads = 128;   // without the quantising warps
+constexpr int kFuseGroups = 4, kFuseThreads = 64 + 64 * kFuseGroups;
 constexpr int kFuseRows = KO_MXFP4_FUSED_ROWS;
 
 template <bool F4, int BN>
@@ -610,7 +612,7 @@ __device__ __forceinline__ void add_slices(const SliceArgs& a, float* part, int 
 }
 
 template <bool F4, int BN, typename T, typename XT>
-__global__ void __launch_bounds__(kSliceThreads)
+__global__ void __launch_bounds__(std::is_void<XT>::value ? kSliceThreads : kFuseThreads)
     slice_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                  const __grid_constant__ CUtensorMap map_sx, const __grid_constant__ CUtensorMap map_sw,
                  const SliceArgs a) {
@@ -635,6 +637,17 @@ __global__ void __launch_bounds__(kSliceThreads)
   const int64_t m0 = static_cast<int64_t>(mt) * BN;
   const int cols = static_cast<int>(min(int64_t(BN), a.M - m0));  // rows of A in this tile
 
+  auto load_stage = [&](int ks, int st) {
+    uint8_t* s = smem + st * C::kStage;
+    mbar_arrive_expect_tx(&full[st], kFuse ? Elem<F4>::kTxW + C::kSf : C::kTx);
+    tma_load_2d(&map_w, &full[st], s, ks * 128, nt * 128);
+    tma_load_2d(&map_sw, &full[st], s + C::kOffSf, ks * 64 * E::kKt, nt);
+    if (!kFuse) {
+      tma_load_2d(&map_x, &full[st], s + C::kW, ks * 128, static_cast<int32_t>(m0));
+      tma_load_2d(&map_sx, &full[st], s + C::kOffSf + C::kSf, ks * 64 * E::kKt, static_cast<int32_t>(m0 / 128));
+    }
+  };
+  const int ahead = min(C::kStages, k1 - k0);  // stages that are loaded before anything else is set up
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], kFuse ? 3 : 1);
@@ -643,15 +656,11 @@ __global__ void __launch_bounds__(kSliceThreads)
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    prefetch_tmap(&map_w);
-    prefetch_tmap(&map_sw);
-    if (!kFuse) {
-      prefetch_tmap(&map_x);
-      prefetch_tmap(&map_sx);
-    }
+    fence_proxy_async_smem();
+    for (int i = 0; i < ahead; ++i) load_stage(k0 + i, i);
   }
   if (kFuse && warp >= 2) {  // the scale tiles of x hold kFuseRows rows; the others are zero for good
-    for (int i = threadIdx.x - 64; i < C::kStages * static_cast<int>(C::kSf / 4); i += 64) {
+    for (int i = threadIdx.x - 64; i < C::kStages * static_cast<int>(C::kSf / 4); i += kFuseThreads - 64) {
       const int st = i / static_cast<int>(C::kSf / 4), w = i % static_cast<int>(C::kSf / 4);
       reinterpret_cast<uint32_t*>(smem + st * C::kStage + C::kOffSf + C::kSf)[w] = 0u;
     }
@@ -668,18 +677,11 @@ __global__ void __launch_bounds__(kSliceThreads)
 
   if (warp == 0) {
     if (lane == 0) {
-      int st = 0, issued = 0;
-      uint32_t phase = 0;
-      for (int ks = k0; ks < k1; ++ks) {
-        if (!mbar_wait(&empty[st], phase ^ 1u, abort_flag)) break;
-        uint8_t* s = smem + st * C::kStage;
-        mbar_arrive_expect_tx(&full[st], kFuse ? Elem<F4>::kTxW + C::kSf : C::kTx);
-        tma_load_2d(&map_w, &full[st], s, ks * 128, nt * 128);
-        tma_load_2d(&map_sw, &full[st], s + C::kOffSf, ks * 64 * E::kKt, nt);
-        if (!kFuse) {
-          tma_load_2d(&map_x, &full[st], s + C::kW, ks * 128, static_cast<int32_t>(m0));
-          tma_load_2d(&map_sx, &full[st], s + C::kOffSf + C::kSf, ks * 64 * E::kKt, static_cast<int32_t>(m0 / 128));
-        }
+      int st = ahead % C::kStages, issued = ahead;
+      uint32_t phase = 0;  // of the MMAs that free a stage
+      for (int ks = k0 + ahead; ks < k1; ++ks) {
+        if (!mbar_wait(&empty[st], phase, abort_flag)) break;
+        load_stage(ks, st);
         ++issued;
         if (++st == C::kStages) {
           st = 0;
@@ -721,42 +723,35 @@ __global__ void __launch_bounds__(kSliceThreads)
     }
     mma_commit_w(acc_full);
   } else if constexpr (kFuse) {
-    // Two blocks of the stage per thread: block b of rows r and r + 8. A block's codes are one 16-byte chunk of the row.
-    const int b = threadIdx.x & 7, r = (threadIdx.x - 64) >> 3;
-    int st = 0;
-    uint32_t phase = 0;
-    for (int ks = k0; ks < k1; ++ks) {
-      uint4 code[2];
-      uint32_t byte[2];
+    // Two blocks of a stage per thread: block b of rows r and r + 8. A block's codes are one 16-byte chunk of the row.
+    const int b = threadIdx.x & 7, r = (threadIdx.x >> 3) & 7;
+    for (int ks = k0 + ((warp - 2) >> 1); ks < k1; ks += kFuseGroups) {
+      Raw8<XT> raw[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        code[i] = make_uint4(0u, 0u, 0u, 0u);
-        byte[i] = 0u;
         const int64_t k = static_cast<int64_t>(ks) * E::kStageK + b * 32;
-        if (r + 8 * i < cols && k < a.K) {
-          const XT* p = static_cast<const XT*>(a.x) + (r + 8 * i) * a.ldx + k;
-          const int left = static_cast<int>(a.K - k);
-          uint32_t c[4];
-          byte[i] = a.x_vec ? quantize_block<XT, KO_MXFP4, true, 1>(p, left, c)
-                            : quantize_block<XT, KO_MXFP4, false, 1>(p, left, c);
-          code[i] = make_uint4(c[0], c[1], c[2], c[3]);
-        }
+        const XT* p = static_cast<const XT*>(a.x) + (r + 8 * i) * a.ldx + k;
+        const int left = r + 8 * i < cols ? static_cast<int>(a.K - k) : 0;
+        if (a.x_vec) load_block<XT, true>(p, left, raw[i]);
+        else load_block<XT, false>(p, left, raw[i]);
       }
+      uint32_t code[2][4], byte[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) byte[i] = quantize_block<XT, KO_MXFP4, 1>(raw[i], code[i]);
+      const int st = (ks - k0) % C::kStages;
+      const uint32_t phase = static_cast<uint32_t>((ks - k0) / C::kStages) & 1u;
       if (!mbar_wait_warp(&empty[st], phase ^ 1u, abort_flag)) break;
       uint8_t* s = smem + st * C::kStage;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = r + 8 * i;
-        *reinterpret_cast<uint4*>(s + C::kW + row * 128 + ((b ^ (row & 7)) << 4)) = code[i];
+        *reinterpret_cast<uint4*>(s + C::kW + row * 128 + ((b ^ (row & 7)) << 4)) =
+            make_uint4(code[i][0], code[i][1], code[i][2], code[i][3]);
         s[C::kOffSf + C::kSf + (b >> 2) * 512 + row * 16 + (b & 3)] = static_cast<uint8_t>(byte[i]);
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[st]);
-      if (++st == C::kStages) {
-        st = 0;
-        phase ^= 1u;
-      }
     }
   }
   __syncwarp();
@@ -769,9 +764,10 @@ __global__ void __launch_bounds__(kSliceThreads)
   T* out = static_cast<T*>(a.out) + m0 * a.N + n;
   float* part = reinterpret_cast<float*>(smem);  // [BN][128]: every load has been read by its MMAs
   const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  const bool epilogue = !kFuse || warp < kSliceThreads / 32;
 #pragma unroll
   for (int c = 0; c < (BN + 31) / 32; ++c) {
-    if (c * 32 >= cols) break;
+    if (c * 32 >= cols || !epilogue) break;
     uint32_t r[32];
     tmem_ld_32x32b_x32(lane_base + c * 32, r);
     tmem_ld_wait_regs(r);
@@ -794,10 +790,10 @@ __global__ void __launch_bounds__(kSliceThreads)
   tc_fence_before();
   if (S > 1) {
     cluster_sync();
-    switch (S) {
-      case 2: add_slices<2, T>(a, part, nt, m0, cols, rank); break;
-      case 4: add_slices<4, T>(a, part, nt, m0, cols, rank); break;
-      default: add_slices<8, T>(a, part, nt, m0, cols, rank); break;
+    if (epilogue) {
+      if (S == 2) add_slices<2, T>(a, part, nt, m0, cols, rank);
+      else if (S == 4) add_slices<4, T>(a, part, nt, m0, cols, rank);
+      else add_slices<8, T>(a, part, nt, m0, cols, rank);
     }
     cluster_sync();  // no CTA leaves while another reads its sums
   } else {
@@ -975,8 +971,11 @@ int launch_slice(const Call& c) {
   a.act = c.act;
   a.k_stages = static_cast<int>((c.Kp + E::kStageK - 1) / E::kStageK);
   a.n_tiles = static_cast<int>(nt);
+  // Slices of K: as many as two CTAs on every SM hold, in clusters of eight only where one on every SM will do (1 x 4096 x
+  // 4096 in 7.3 us with eight, 6.7 with four; 1 x 8192 x 1024 in 6.7 and 9.0).
   int slices = 1;
-  while (slices < 8 && mt * nt * slices * 2 <= 2 * c.info->sm_count && slices * 2 <= a.k_stages) slices *= 2;
+  while (slices < 8 && mt * nt * slices * 2 <= (slices == 4 ? 1 : 2) * c.info->sm_count && slices * 2 <= a.k_stages)
+    slices *= 2;
   a.slices = slices;
   a.vec_out = c.N % 4 == 0 && reinterpret_cast<uintptr_t>(c.out) % (4 * sizeof(T)) == 0;
   auto kernel = slice_kernel<F4, BN, T, XT>;
@@ -984,7 +983,8 @@ int launch_slice(const Call& c) {
   rc = allow_smem(kernel, allowed, current_device(), C::kSmem);
   if (rc) return rc;
   cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = cluster_config(attr, slices, static_cast<unsigned>(mt * nt * slices), kSliceThreads, C::kSmem,
+  cudaLaunchConfig_t cfg = cluster_config(attr, slices, static_cast<unsigned>(mt * nt * slices),
+                                          kFuse ? kFuseThreads : kSliceThreads, C::kSmem,
                                           c.stream);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, msx, msw, a);
   if (e != cudaSuccess) return ko::fail(static_cast<int>(e), std::string(who) + ": launch failed");
