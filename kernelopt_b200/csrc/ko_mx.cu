@@ -155,6 +155,17 @@ __global__ void __launch_bounds__(kThreads) pack_weight_kernel(const T* __restri
 // the 128 elements of a scale word, so a quantised block costs two shuffles and its scales are stored a word at a time. OUT: -1 writes y in the input's type, else
 // the MX format.
 // ---------------------------------------------------------------------------------------------------------
+// 1 / sqrt(x) as the sum of two fp32 numbers: the special-function value r and one Newton step's correction, r (1 - x r^2)
+// / 2, with r^2 kept exactly. y then has the roundings of v * gamma and of the product only, which decides how many 8-bit
+// codes next to a border come out on the other side. Where r^2 could leave the range, r is the rounded value alone.
+__device__ __forceinline__ float2 inverse_root(float x) {
+  if (!(x > 1e-30f && x < 1e30f)) return make_float2(1.0f / sqrtf(x), 0.f);
+  const float r = rsqrtf(x), t = r * r;
+  const float rest = fmaf(-x, t, 1.0f) - x * fmaf(r, r, -t);
+  return make_float2(r, 0.5f * r * rest);
+}
+__device__ __forceinline__ float scaled(float p, float2 r) { return fmaf(p, r.y, p * r.x); }
+
 struct NormArgs {
   const void *h, *o, *bias, *scale, *gamma;
   void *h_out, *y;
@@ -241,7 +252,7 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kerne
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   }
-  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.C) + a.eps);
+  const float2 rstd = inverse_root(sum / static_cast<float>(a.C) + a.eps);
   if constexpr (OUT < 0) {
     if (!real) return;
     T* y = static_cast<T*>(a.y) + row * a.C + t * 8;
@@ -250,7 +261,7 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kerne
       float gm[8];
       widen8(g[i], gm);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gm[j] *= v[i][j] * rstd;
+      for (int j = 0; j < 8; ++j) gm[j] = scaled(v[i][j] * gm[j], rstd);
       store8<T, VEC>(y + i * kStep, left - i * kStep, gm);
     }
   } else {
@@ -270,7 +281,7 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kerne
       // beyond C v is 0, and 0 * rstd would be NaN for an infinite rstd (eps 0, a row of zeros)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        gm[j] *= v[i][j] * rstd;
+        gm[j] = scaled(v[i][j] * gm[j], rstd);
         if (VEC ? left - i * kStep <= 0 : j >= left - i * kStep) gm[j] = 0.f;
       }
       quantize_group<OUT>(gm, amax_bits8(gm), 0xffffu << (threadIdx.x & 16), code + i * TPR * kBytes,

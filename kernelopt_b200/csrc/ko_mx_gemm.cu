@@ -11,7 +11,8 @@
 // them over tensor memory, ahead of the stage's MMAs on the same pipe.
 //
 // Two kernels: pairs of CTAs with tiles of 256 rows for many rows (pair_kernel), and single CTAs over slices of K for few
-// (slice_kernel); launch() says which takes a product. Every wait is bounded; a wait that runs out ends the kernel with KO_ERR_DEVICE_TIMEOUT in *dev_status.
+// (slice_kernel); launch() says which takes a product. Every wait is bounded; a wait that runs out ends the kernel with
+// KO_ERR_DEVICE_TIMEOUT in *dev_status.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -105,7 +106,7 @@ __device__ __forceinline__ float4 cluster_load_f4(uint32_t addr) {
 }
 // Arrive on a barrier of the pair's leader. What the arrival orders are tensor-memory reads, before the MMAs that the leader
 // issues next, and the tcgen05 fences on both sides see to that; a release at cluster scope, a memory barrier across the
-// pair, made each tile's hand-over a microsecond longer.
+// pair, made each tile's hand-over half a microsecond longer (25664 x 128 x 1536 28.4 -> 20.8 us).
 __device__ __forceinline__ void arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -149,8 +150,9 @@ __device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
 // on [0, 6] (it falls from 1/2 to 0.066), so a polynomial of degree 12 in |v| / 3 - 1 has it, fitted by least squares at
 // Chebyshev nodes: q is within 3e-5 of itself everywhere, so the far negative side keeps its small values, and |v| q
 // within 8e-8. Beyond 6, g stays at its last value; q is below 1e-9 there. NaN stays NaN, and GELU(-inf) is 0, its limit.
-// Without a division, it costs one special-function instruction; A&S 7.1.26 (two of them, no packed form) took 30 us more
-// of the 25664 x 1536 fp32 outputs of the backbone's fc1.
+// It costs one special-function instruction, and all else but the ends is packed: 25664 x 384 x 1536 with fp32 outputs takes
+// 34 us without an activation and 41 with this one. A&S 7.1.26 as the fp32-grade GEMM has it (two special-function
+// instructions, not packed) added 30 us to the same product at an earlier state of the epilogue.
 __device__ __forceinline__ void gelu_pair(float& a, float& b) {
   constexpr float g[13] = {-0.12151393294334412f, 0.10320935398340225f, -0.08236773312091827f, 0.062280356884002686f,
                            -0.04567015543580055f, 0.03141380101442337f, -0.01772490330040455f, 0.013943932950496674f,
