@@ -186,52 +186,77 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kerne
   const bool real = row < a.rows;
   const int left = real ? static_cast<int>(a.C) - t * 8 : 0;  // elements from this thread's first one to the row's end
   constexpr int kStep = TPR * 8;
+  // All loads of a row go out before the arithmetic, gamma's while the sum is taken. The widest rows of fp32 have no
+  // registers for that with the block's 1024 threads: they take group after group (2048 x 32768: 171 us, 470 otherwise).
+  constexpr bool kAhead = !(sizeof(T) == 4 && TPR * NV > 2048);
+  constexpr int kHold = kAhead ? NV : 1;
   float v[NV][8];
+  Raw8<T> g[kHold];
+  auto group = [&](const void* p, int i) {
+    return load8<T, VEC>(static_cast<const T*>(p) + t * 8 + i * kStep, left - i * kStep);
+  };
   {
-    const T* h = static_cast<const T*>(a.h) + row * a.ldh + t * 8;
-    Raw8<T> r[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) r[i] = load8<T, VEC>(h + i * kStep, left - i * kStep);
-    if (a.o) {
-      const T* o = static_cast<const T*>(a.o) + row * a.ldo + t * 8;
-      Raw8<T> q[NV];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) q[i] = load8<T, VEC>(o + i * kStep, left - i * kStep);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) widen8(q[i], v[i]);
+    const T* h = static_cast<const T*>(a.h) + row * a.ldh;
+    const T* o = a.o ? static_cast<const T*>(a.o) + row * a.ldo : nullptr;
+    // v[i], the widened o, becomes (o + bias) * scale for the groups [from, to); one branch for all of them
+    auto affine = [&](auto from, auto to) {
+      float x[8];
       if (a.bias) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float b[8];
-          widen8(load8<T, VEC>(static_cast<const T*>(a.bias) + t * 8 + i * kStep, left - i * kStep), b);
+        for (int i = from; i < to; ++i) {
+          widen8(group(a.bias, i), x);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] += b[j];
+          for (int j = 0; j < 8; ++j) v[i][j] += x[j];
         }
       }
       if (a.scale) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float s[8];
-          widen8(load8<T, VEC>(static_cast<const T*>(a.scale) + t * 8 + i * kStep, left - i * kStep), s);
+        for (int i = from; i < to; ++i) {
+          widen8(group(a.scale, i), x);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] *= s[j];
+          for (int j = 0; j < 8; ++j) v[i][j] *= x[j];
         }
       }
+    };
+    auto add = [&](int i, const Raw8<T>& hr) {
+      float x[8];
+      widen8(hr, x);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float x[8];
-        widen8(r[i], x);
+      for (int j = 0; j < 8; ++j) v[i][j] += x[j];
+    };
+    if constexpr (kAhead) {
+      Raw8<T> r[NV], q[NV];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] += x[j];
+      for (int i = 0; i < NV; ++i) r[i] = group(h, i);
+      if (o) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = group(o, i);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) widen8(q[i], v[i]);
+        affine(0, NV);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) add(i, r[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) widen8(r[i], v[i]);
       }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) g[i] = group(a.gamma, i);
     } else {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) widen8(r[i], v[i]);
+      for (int i = 0; i < NV; ++i) {
+        const Raw8<T> r = group(h, i);
+        if (o) {
+          widen8(group(o, i), v[i]);
+          affine(i, i + 1);
+          add(i, r);
+        } else {
+          widen8(r, v[i]);
+        }
+      }
     }
   }
-  Raw8<T> g[NV];  // on its way while the sum is taken
-#pragma unroll
-  for (int i = 0; i < NV; ++i) g[i] = load8<T, VEC>(static_cast<const T*>(a.gamma) + t * 8 + i * kStep, left - i * kStep);
+  auto gamma_of = [&](int i) { return kAhead ? g[kAhead ? i : 0] : group(a.gamma, i); };
   if (a.h_out) {
     T* h_out = static_cast<T*>(a.h_out) + row * a.C + t * 8;
 #pragma unroll
@@ -259,7 +284,7 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kerne
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float gm[8];
-      widen8(g[i], gm);
+      widen8(gamma_of(i), gm);
 #pragma unroll
       for (int j = 0; j < 8; ++j) gm[j] = scaled(v[i][j] * gm[j], rstd);
       store8<T, VEC>(y + i * kStep, left - i * kStep, gm);
@@ -277,7 +302,7 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kerne
         continue;
       }
       float gm[8];
-      widen8(g[i], gm);
+      widen8(gamma_of(i), gm);
       // beyond C v is 0, and 0 * rstd would be NaN for an infinite rstd (eps 0, a row of zeros)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -301,11 +326,16 @@ int launch_norm(const NormArgs& a, cudaStream_t s) {
 
 template <typename T, int OUT, bool VEC>
 int pick_norm(const NormArgs& a, cudaStream_t s) {
+  // Two groups of eight to a thread (16 threads with three of them up to 384, a multiple of what 32 threads would hold idle):
+  // 16384 x 4096 in 127 us fp32 and 78 us bf16, 130 and 80 with half the threads, 127 and 92 with twice as many; one row
+  // of 4096 in 2.4 us, 2.8 and 2.4. From 8192 on the threads of a block bound it: 8192 x 16384 bf16 in 148 us with 512
+  // threads and four groups, 212 with 1024 and two.
   if (a.C <= 384) return launch_norm<T, OUT, VEC, 16, 3>(a, s);
-  if (a.C <= 1024) return launch_norm<T, OUT, VEC, 32, 4>(a, s);
-  if (a.C <= 2048) return launch_norm<T, OUT, VEC, 64, 4>(a, s);
-  if (a.C <= 4096) return launch_norm<T, OUT, VEC, 128, 4>(a, s);
-  if (a.C <= 8192) return launch_norm<T, OUT, VEC, 256, 4>(a, s);
+  if (a.C <= 512) return launch_norm<T, OUT, VEC, 32, 2>(a, s);
+  if (a.C <= 1024) return launch_norm<T, OUT, VEC, 64, 2>(a, s);
+  if (a.C <= 2048) return launch_norm<T, OUT, VEC, 128, 2>(a, s);
+  if (a.C <= 4096) return launch_norm<T, OUT, VEC, 256, 2>(a, s);
+  if (a.C <= 8192) return launch_norm<T, OUT, VEC, 512, 2>(a, s);
   if (a.C <= 16384) return launch_norm<T, OUT, VEC, 512, 4>(a, s);
   return launch_norm<T, OUT, VEC, 1024, 4>(a, s);
 }
