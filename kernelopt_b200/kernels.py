@@ -601,8 +601,6 @@ def _rows(t, name, dtype=None, device=None):
 
 
 def _vector(t, name, width, dtype, device):
-    if t is None:
-        return None
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
         raise ValueError(f"{name} must be a CUDA tensor on {device}")
     if t.dtype != dtype or t.numel() != width or not t.is_contiguous():
@@ -630,9 +628,10 @@ class MXTensor:
         # of 128 is, in rows of codes, a 32nd (mxfp8) or a 16th (mxfp4) of the tiles' rows.
         kp, tile_rows = -(-k // 128) * 128, -(-rows // 128) * 128
         if fmt == "mxfp4":
-            self.buf = _dense((rows + tile_rows // 16, kp // 2), torch.uint8, device)
+            size, stride, dt = (rows + tile_rows // 16, kp // 2), (kp // 2, 1), torch.uint8
         else:
-            self.buf = _dense((rows + tile_rows // 32, kp), torch.float8_e4m3fn, device)
+            size, stride, dt = (rows + tile_rows // 32, kp), (kp, 1), torch.float8_e4m3fn
+        self.buf = torch.empty_strided(size, stride, dtype=dt, device=device)
 
     @property
     def device(self):
@@ -682,11 +681,11 @@ def residual_rmsnorm(h, o, bias, scale, gamma, eps, quantize=None, h_out=None):
     apart from both); y
     too, or with quantize "mxfp8" / "mxfp4" as an MXTensor, quantised from fp32 in the same pass."""
     rows, ldh = _rows(h, "h")
-    if o.shape != h.shape:
+    if not isinstance(o, torch.Tensor) or o.shape != h.shape:
         raise ValueError("h and o must have the same shape")
     _, ldo = _rows(o, "o", h.dtype, h.device)
     if h_out is None:
-        h_out = _dense(h.shape, h.dtype, h.device)
+        h_out = torch.empty_like(h) if h.is_contiguous() else _dense(h.shape, h.dtype, h.device)
     elif h_out.shape != h.shape or h_out.dtype != h.dtype or h_out.device != h.device or not h_out.is_contiguous():
         raise ValueError("h_out must be contiguous, of h's shape, type and device")
     return h_out, _rmsnorm(h, rows, ldh, o.data_ptr(), ldo, bias, scale, gamma, eps, quantize, h_out.data_ptr())
@@ -702,10 +701,10 @@ def _rmsnorm(h, rows, ldh, o_ptr, ldo, bias, scale, gamma, eps, quantize, h_out_
     c, dt, dev = h.shape[-1], h.dtype, h.device
     if gamma is None:
         raise ValueError("gamma is required")
-    params = (_vector(bias, "bias", c, dt, dev), _vector(scale, "scale", c, dt, dev),
-              _vector(gamma, "gamma", c, dt, dev))
+    params = (None if bias is None else _vector(bias, "bias", c, dt, dev),
+              None if scale is None else _vector(scale, "scale", c, dt, dev), _vector(gamma, "gamma", c, dt, dev))
     if quantize is None:
-        y = _dense(h.shape, dt, dev)
+        y = torch.empty_like(h) if h.is_contiguous() else _dense(h.shape, dt, dev)
         to = (y.data_ptr(), 0, None, None)
     else:
         y = MXTensor(h.shape, quantize, dt, dev)
