@@ -10,7 +10,10 @@ below a last place of the largest term: 2^-22 of the sum of magnitudes S per ste
 """
 from __future__ import annotations
 
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -21,6 +24,7 @@ from kernelopt_b200 import _lib
 from kernelopt_b200 import kernels as K
 
 pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parent.parent
 
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}  # a subnormal's step
@@ -286,7 +290,7 @@ def check_linear(got, a, w, bias, act, what=""):
 SHAPES = [(1, 1, 1), (1, 32, 8), (3, 33, 5), (127, 128, 129), (128, 256, 128), (129, 320, 257), (300, 1000, 517),
           (1, 4096, 1024), (2, 2048, 100), (65, 64, 1024), (16, 512, 384), (9, 8192, 72), (513, 1152, 640),
           (1000, 384, 1536), (1111, 700, 2049), (5001, 300, 2560), (300, 136, 5003), (700, 1300, 2601),
-          (2600, 1100, 4704)]
+          (2600, 1100, 4704), (700, 96, 8), (2000, 40, 12), (600, 4096, 16), (100, 8192, 260), (90, 512, 1000)]
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -332,7 +336,7 @@ def test_linear_fused_rows(cuda, m, dtype):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("m", [1, 40, 200])
+@pytest.mark.parametrize("m", [1, 40, 200, 600])
 def test_linear_rows_do_not_meet(cuda, m, fmt):
     """A row or a weight column that is not finite stays in its own outputs, rows of zeros give the bias, and what lies
     behind the output is left as it was."""
@@ -470,9 +474,10 @@ def test_layer_run(cuda, dtype, rows):
     check_linear(out, OM.round_trip(np64(m), "mxfp4"), np64(p2.dequantize()), np64(b2), None, "down")
 
 
-def test_streams_threads_and_graphs(cuda):
+@pytest.mark.parametrize("rows", [5, 50, 700])
+def test_streams_threads_and_graphs(cuda, rows):
     """The same results on another stream, from two threads at once, and captured into graphs that run side by side."""
-    c, n, rows = 512, 640, 50
+    c, n = 512, 640
     h, o, _, _, gamma = norm_inputs(rows, c, 41, torch.bfloat16, cuda, False)
     w, b = weight(c, n, 42, torch.bfloat16, cuda)
     pw = K.pack_weight_mxfp4(w, b)
@@ -523,6 +528,37 @@ def test_streams_threads_and_graphs(cuda):
     torch.cuda.synchronize()
     assert all(torch.equal(a, x) for a, x in zip(outs[0], want)) and all(torch.equal(a, x) for a, x in zip(outs[1], want2))
     K.check_device_status(cuda)
+
+
+FIRST_IN_CAPTURE = """
+import torch
+from kernelopt_b200 import kernels as K
+g = torch.cuda.CUDAGraph()
+x = torch.randn(ROWS, 512, device="cuda")
+pw = K.pack_weight_mxfp4(torch.randn(512, 640, device="cuda"))
+gamma = torch.ones(512, device="cuda")
+s = torch.cuda.Stream()
+torch.cuda.synchronize()
+with torch.cuda.graph(g, stream=s):
+    v, y = K.residual_rmsnorm(x, x, None, None, gamma, 1e-6, quantize="mxfp8")
+    a, b = K.linear_mxfp4(y, pw, "gelu"), K.linear_mxfp4(v, pw)
+    d = y.dequantize()
+g.replay()
+torch.cuda.synchronize()
+v2, y2 = K.residual_rmsnorm(x, x, None, None, gamma, 1e-6, quantize="mxfp8")
+assert torch.equal(v, v2) and torch.equal(d, y2.dequantize())
+assert torch.equal(a, K.linear_mxfp4(y2, pw, "gelu")) and torch.equal(b, K.linear_mxfp4(v2, pw))
+K.check_device_status()
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("rows", [3, 40, 700])
+def test_first_call_inside_a_capture(cuda, rows):
+    """A process whose first use of the kernels is being captured."""
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE.replace("ROWS", str(rows))], capture_output=True, text=True,
+                       timeout=300, cwd=ROOT)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_launch_counts(cuda):
