@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const T* __restrict_
                                                             int64_t ldx, int64_t items, uint32_t kblocks,
                                                             int64_t code_pitch, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales) {
+  let_next_grid_start();  // the product behind it sets itself up meanwhile (ko_linear_quantize_mxfp4)
   // items: a multiple of 512 blocks, so every warp is whole, in range or not, and the lanes of a block stay together
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
   if (item >= items) return;
@@ -256,7 +257,10 @@ __global__ void __launch_bounds__(TPR > kThreads ? TPR : kThreads) rmsnorm_kerne
       }
     }
   }
-  auto gamma_of = [&](int i) { return kAhead ? g[kAhead ? i : 0] : group(a.gamma, i); };
+  auto gamma_of = [&](int i) {
+    if constexpr (kAhead) return g[i];
+    else return group(a.gamma, i);
+  };
   if (a.h_out) {
     T* h_out = static_cast<T*>(a.h_out) + row * a.C + t * 8;
 #pragma unroll

@@ -31,6 +31,12 @@ constexpr int64_t kMaxK = int64_t(1) << 24;
 
 #if defined(__CUDACC__)
 
+// Programmatic dependent launch: a kernel that is launched behind another one may set itself up while the other's last CTAs
+// run, and waits here, before it touches global memory, until that grid is complete and what it wrote is visible.
+__device__ __forceinline__ void wait_for_previous_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets such a kernel be launched once every CTA of this grid has come here.
+__device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
