@@ -1000,15 +1000,15 @@ int launch_slice(const Call& c) {
   return ko::check_launch(who);
 }
 
-// Which kernel, by the numbers of 256 x 128 tiles and of pipeline stages along K (bf16 outputs, us on B200):
-//   up to 64 rows, the slices: 48 x 8192 x 8192 in 10.1 against 15.3 with pairs.
+// Which kernel, by the numbers of 256 x 128 tiles and of pipeline stages along K (mxfp4, bf16 outputs, us on B200):
+//   up to 64 rows, the slices: 48 x 8192 x 8192 in 9.9 against 14.8 with pairs.
 //   More rows and fewer tiles than stages, the slices too, for the pairs would leave most SMs idle behind a long K:
-//   300 x 4096 x 512 in 8.0 against 9.9; with more tiles, the pairs: 1200 x 4096 x 512 in 10.0 against 10.6 and
-//   1200 x 1024 x 1024 in 6.6 against 8.4. One tile of 128 rows reads the weight once, and the slices keep a long K
-//   longer: 128 x 8192 x 8192 in 13.1 against 15.9.
-//   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.7 against 11.6) or K is at
-//   most two stages, where the epilogue counts (25664 x 384 x 1536 in 24.1 against 29.5); else 256 x 256, with less to
-//   load for a product (25664 x 1024 x 1536 in 29.3 against 34.4, 8192 x 4096 x 8192 in 111 against 149).
+//   300 x 4096 x 512 in 7.8 against 9.8; with more tiles, the pairs: 1200 x 4096 x 512 in 10.0 against 10.7 and
+//   1200 x 1024 x 1024 in 6.7 against 8.2. One tile of 128 rows reads the weight once, and there the slices keep a long K
+//   longer: 128 x 4096 x 4096 in 9.1 against 10.2.
+//   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.5 against 11.6) or K is at
+//   most two stages, where the epilogue counts (25664 x 384 x 1536 with GELU in 39 against 44); else 256 x 256, with less
+//   to load for a product (25664 x 1024 x 1536 in 30 against 34, 4096 x 8192 x 8192 in 98 against 141).
 template <bool F4, typename T>
 int launch(const Call& c) {
   const int64_t tiles = ((c.M + 255) / 256) * ((c.N + 127) / 128);
@@ -1016,7 +1016,7 @@ int launch(const Call& c) {
   if (c.M <= 16) return launch_slice<F4, 16, T>(c);
   if (c.M <= 32) return launch_slice<F4, 32, T>(c);
   if (c.M <= 64) return launch_slice<F4, 64, T>(c);
-  if (tiles <= stages || (c.M <= 128 && stages >= 32)) return launch_slice<F4, 128, T>(c);
+  if (tiles <= stages || (c.M <= 128 && stages >= 16)) return launch_slice<F4, 128, T>(c);
   if (tiles <= c.info->sm_count / 2 || stages <= 2) return launch_pair<F4, 128, T>(c);
   return launch_pair<F4, 256, T>(c);
 }

@@ -678,15 +678,15 @@ def residual_rmsnorm(h, o, bias, scale, gamma, eps, quantize=None, h_out=None):
     (width <= 32768), both computed in fp32: residual_layernorm's arguments for a model that normalises by the root
     mean square. h and o: [..., C] float32, bfloat16 or float16 (any even row pitch); bias and scale [C] or None (0 / 1);
     gamma [C]; all of one type. v is returned in that type, in h_out where given ([..., C] contiguous; h or o itself, or
-    apart from both); y
-    too, or with quantize "mxfp8" / "mxfp4" as an MXTensor, quantised from fp32 in the same pass."""
+    apart from both). y has that type too, or is with quantize "mxfp8" / "mxfp4" an MXTensor, quantised from fp32 in the
+    same pass."""
     rows, ldh = _rows(h, "h")
     if not isinstance(o, torch.Tensor) or o.shape != h.shape:
         raise ValueError("h and o must have the same shape")
     _, ldo = _rows(o, "o", h.dtype, h.device)
     if h_out is None:
         h_out = torch.empty_like(h) if h.is_contiguous() else _dense(h.shape, h.dtype, h.device)
-    elif h_out.shape != h.shape or h_out.dtype != h.dtype or h_out.device != h.device or not h_out.is_contiguous():
+    elif not isinstance(h_out, torch.Tensor) or h_out.shape != h.shape or h_out.dtype != h.dtype or h_out.device != h.device or not h_out.is_contiguous():
         raise ValueError("h_out must be contiguous, of h's shape, type and device")
     return h_out, _rmsnorm(h, rows, ldh, o.data_ptr(), ldo, bias, scale, gamma, eps, quantize, h_out.data_ptr())
 
@@ -749,7 +749,8 @@ def pack_weight_mxfp4(w, bias=None) -> PackedWeightMX:
 def linear_mxfp4(x, pw: PackedWeightMX, act=None, out_dtype=None, out=None):
     """act(x @ W + bias) with W in mxfp4, on the block-scaled tensor-core products with fp32 accumulation. x: an
     MXTensor [..., K] (mxfp8 or mxfp4), or a float32 / bfloat16 / float16 tensor, which is quantised to mxfp4 (up to 16
-    rows inside the product's kernel, more in a pass before it). act None, 'gelu' or 'relu'. The output [..., N] is rounded once, to out_dtype (x's type by default)."""
+    rows inside the product's kernel, more in a pass before it). act None, 'gelu' or 'relu'. The output [..., N] is rounded
+    once, to out_dtype (x's type by default). out, where given, is contiguous and does not overlap x."""
     if act not in ACTS:
         raise ValueError(f"act must be one of {list(ACTS)}")
     wdev = pw.mx.buf.device
