@@ -155,9 +155,9 @@ __global__ void __launch_bounds__(kThreads) pack_weight_kernel(const T* __restri
 // Residual + root-mean-square norm. T threads share a row and keep its NV groups of eight elements each in fp32
 // registers from the load to the store, so h and o are read once; the sum of squares is a shuffle tree and, for rows of
 // more than a warp, one exchange through shared memory, both in a fixed order. Four lanes hold a block of 32 and sixteen
-// the 128 elements of a scale word, so a quantised block costs two shuffles and its scales are stored a word at a time. Bound
-// by HBM: 16384 x 8192 bf16 to mxfp8 in 153 us (6.2 TB/s; 68 % of the issue slots), 25664 x 384 fp32 in 20 to 24. OUT: -1 writes y in the input's type, else
-// the MX format.
+// the 128 elements of a scale word, so a quantised block costs two shuffles and its scales are stored a word at a time.
+// Bound by HBM: 16384 x 8192 bf16 to mxfp8 in 153 us (6.2 TB/s; 68 % of the issue slots), 25664 x 384 fp32 in 20 to 24 us.
+// OUT: -1 writes y in the input's type, else the MX format.
 // ---------------------------------------------------------------------------------------------------------
 // 1 / sqrt(x) as the sum of two fp32 numbers: the special-function value r and one Newton step's correction, r (1 - x r^2)
 // / 2, with r^2 kept exactly. y then has the roundings of v * gamma and of the product only, which decides how many 8-bit
@@ -333,10 +333,13 @@ int launch_norm(const NormArgs& a, cudaStream_t s) {
 
 template <typename T, int OUT, bool VEC>
 int pick_norm(const NormArgs& a, cudaStream_t s) {
-  // Two groups of eight to a thread (16 threads with three of them up to 384, a multiple of what 32 threads would hold idle):
-  // 16384 x 4096 in 127 us fp32 and 78 us bf16, 130 and 80 with half the threads, 127 and 92 with twice as many; one row
-  // of 4096 in 2.4 us, 2.8 and 2.4. From 8192 on the threads of a block bound it: 8192 x 16384 bf16 in 148 us with 512
-  // threads and four groups, 212 with 1024 and two.
+  // Half a warp to a row up to 384 (102656 x 384 in 76 us fp32 and 44 us bf16; 75 and 54 with a warp of two groups to a
+  // thread), with no more groups than the row has. Then two groups of eight to a thread: 16384 x 4096 in 127 us fp32 and
+  // 78 us bf16, 130 and 80 with half the threads, 127 and 92 with twice as many; one row of 4096 in 2.4 us, 2.8 and 2.4.
+  // From 8192 on the threads of a block bound it: 8192 x 16384 bf16 in 148 us with 512 threads and four groups, 212 with
+  // 1024 and two.
+  if (a.C <= 128) return launch_norm<T, OUT, VEC, 16, 1>(a, s);
+  if (a.C <= 256) return launch_norm<T, OUT, VEC, 16, 2>(a, s);
   if (a.C <= 384) return launch_norm<T, OUT, VEC, 16, 3>(a, s);
   if (a.C <= 512) return launch_norm<T, OUT, VEC, 32, 2>(a, s);
   if (a.C <= 1024) return launch_norm<T, OUT, VEC, 64, 2>(a, s);

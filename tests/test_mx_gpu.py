@@ -183,7 +183,8 @@ def check_norm_quantized(q, y, dy, what=""):
 @pytest.mark.parametrize("rows,c,affine", [(1, 1, False), (1, 32, True), (5, 33, True), (130, 384, True),
                                            (17, 385, False), (33, 1000, True), (3, 1024, False), (5, 1025, True),
                                            (9, 2048, False), (4, 4095, True), (2, 4096, False), (3, 8192, True),
-                                           (2, 8200, False), (2, 16392, False), (1, 32768, True), (300, 128, False)])
+                                           (2, 8200, False), (2, 16392, False), (1, 32768, True), (300, 128, False),
+                                           (41, 200, True), (6, 256, False), (9, 512, True)])
 def test_residual_rmsnorm(cuda, rows, c, affine, dtype, out):
     args = norm_inputs(rows, c, rows + c, dtype, cuda, affine)
     v, dv, y, dy = norm_oracle(*args, 1e-6)
