@@ -1008,9 +1008,10 @@ int launch_slice(const Call& c) {
 //   300 x 4096 x 512 in 7.8 against 9.8; with more tiles, the pairs: 1200 x 4096 x 512 in 10.0 against 10.7 and
 //   1200 x 1024 x 1024 in 6.7 against 8.2. One tile of 128 rows reads the weight once, and there the slices keep a long K
 //   longer: 128 x 4096 x 4096 in 9.1 against 10.2.
-//   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.5 against 11.6) or K is at
-//   most two stages, where the epilogue counts (25664 x 384 x 1536 with GELU in 39 against 44); else 256 x 256, with less
-//   to load for a product (25664 x 1024 x 1536 in 30 against 34, 4096 x 8192 x 8192 in 98 against 141).
+//   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.5 against 11.6) or K is so
+//   short that the epilogue counts: two stages (25664 x 512 x 1536 in 24.3 against 24.7), four with GELU (25664 x 1024 x
+//   1536 in 43 against 47; without, 34 against 30). Else 256 x 256, with less to load for a product (25664 x 2048 x 1536
+//   with GELU in 53 against 61, 4096 x 8192 x 8192 in 98 against 141).
 template <bool F4, typename T>
 int launch(const Call& c) {
   const int64_t tiles = ((c.M + 255) / 256) * ((c.N + 127) / 128);
@@ -1019,7 +1020,7 @@ int launch(const Call& c) {
   if (c.M <= 32) return launch_slice<F4, 32, T>(c);
   if (c.M <= 64) return launch_slice<F4, 64, T>(c);
   if (tiles <= stages || (c.M <= 128 && stages >= 16)) return launch_slice<F4, 128, T>(c);
-  if (tiles <= c.info->sm_count / 2 || stages <= 2) return launch_pair<F4, 128, T>(c);
+  if (tiles <= c.info->sm_count / 2 || stages <= (c.act == KO_ACT_GELU ? 4 : 2)) return launch_pair<F4, 128, T>(c);
   return launch_pair<F4, 256, T>(c);
 }
 
