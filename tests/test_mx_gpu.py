@@ -291,7 +291,8 @@ def check_linear(got, a, w, bias, act, what=""):
 SHAPES = [(1, 1, 1), (1, 32, 8), (3, 33, 5), (127, 128, 129), (128, 256, 128), (129, 320, 257), (300, 1000, 517),
           (1, 4096, 1024), (2, 2048, 100), (65, 64, 1024), (16, 512, 384), (9, 8192, 72), (513, 1152, 640),
           (1000, 384, 1536), (1111, 700, 2049), (5001, 300, 2560), (300, 136, 5003), (700, 1300, 2601),
-          (2600, 1100, 4704), (700, 96, 8), (2000, 40, 12), (600, 4096, 16), (100, 8192, 260), (90, 512, 1000)]
+          (2600, 1100, 4704), (700, 96, 8), (2000, 40, 12), (600, 4096, 16), (100, 8192, 260), (90, 512, 1000),
+          (1500, 1300, 2051), (1501, 1300, 2056)]
 
 
 @pytest.mark.parametrize("fmt", FMTS)
