@@ -95,11 +95,11 @@ struct AttnCfg {
   static constexpr uint32_t kOffK = 2 * kQBytes;               // two k buffers (block j in buffer j & 1)
   static constexpr uint32_t kOffV = kOffK + 2 * kKBufBytes;    // two v buffers
   static constexpr uint32_t kOffBars = kOffV + 2 * kVBufBytes;
-  // At least 120 KB even where the tiles need less (head dim 32), so that one CTA per SM holds all 512 tensor-
-  // memory columns and no second CTA waits in tcgen05.alloc.
+  // More than the tiles need at head dim 32, so that one CTA per SM holds all 512 tensor-memory columns and no
+  // second CTA, of this kernel or another, waits in tcgen05.alloc.
   static constexpr uint32_t kOffRowPtr = kOffBars + 256;  // [BQ] output-row pointers of the softmax threads
   static constexpr size_t kSmemNeed = 1024 + kOffRowPtr + BQ * 8;
-  static constexpr size_t kSmemBytes = kSmemNeed > 120 * 1024 ? kSmemNeed : 120 * 1024;
+  static constexpr size_t kSmemBytes = kSmemNeed > ko::kWholeTmemSmem ? kSmemNeed : ko::kWholeTmemSmem;
   static_assert(HD == 32 || HD == 64, "head dim 32 or 64");
 };
 

@@ -9,6 +9,7 @@
 #include <string>
 
 #include "../../include/kernelopt.h"
+#include "ko_residency.h"
 
 namespace ko {
 

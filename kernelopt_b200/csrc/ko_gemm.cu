@@ -110,6 +110,7 @@ struct Cfg {
   static constexpr uint32_t kLayout = BKB == 128 ? 2u : 4u;  // descriptor layout: 128B / 64B swizzle
   static_assert(kStages >= 2, "stage does not fit");
   static_assert(kTmemNeed <= 512, "TMEM overflow");
+  static_assert(kSmemBytes >= ko::kWholeTmemSmem, "a CTA has its SM, and all of its tensor memory, to itself");
   static_assert((4 * kStages + 10) * 8 <= kBarBytes, "barrier area");
 };
 

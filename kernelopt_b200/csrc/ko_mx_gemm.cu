@@ -11,8 +11,9 @@
 // them over tensor memory, ahead of the stage's MMAs on the same pipe.
 //
 // Two kernels: pairs of CTAs with tiles of 256 rows for many rows (pair_kernel), and single CTAs over slices of K for few
-// (slice_kernel); launch() says which takes a product. Every wait is bounded; a wait that runs out ends the kernel with
-// KO_ERR_DEVICE_TIMEOUT in *dev_status.
+// (slice_kernel); launch() says which takes a product. Every wait on a barrier in shared memory is bounded; one that runs out
+// ends the kernel with KO_ERR_DEVICE_TIMEOUT in *dev_status. The allocation of tensor memory and the cluster's own barrier have
+// no limit: ko_residency.h keeps the first from waiting for another kernel.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -20,6 +21,7 @@
 #include <type_traits>
 
 #include "ko_mx.cuh"
+#include "ko_mx_cfg.h"
 
 namespace {
 
@@ -111,20 +113,6 @@ __device__ __forceinline__ void arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-template <bool F4>
-struct Elem {
-  static constexpr uint32_t kTypeA = F4 ? 1u : 0u;  // e2m1 / e4m3
-  static constexpr uint32_t kTypeW = F4 ? 1u : 5u;  // e2m1 in either kind's numbering
-  static constexpr int kStageK = F4 ? 256 : 128;    // elements along K per stage: 128 bytes of shared memory per row
-  static constexpr int kKt = kStageK / 128;         // scale tiles along K per stage
-  static constexpr int kMma = 4;                    // instructions along K per stage, 32 bytes each
-  // What a barrier counts for a box of 128 weight rows: the bytes that TMA reads. A spread box reads half of what it fills.
-  static constexpr uint32_t kTxW = 128 * (F4 ? 128 : 64);
-  // scale word (tile along K) and first scale byte of instruction j
-  static constexpr __host__ __device__ int kt_of(int j) { return F4 ? j >> 1 : 0; }
-  static constexpr __host__ __device__ uint32_t sf_of(int j) { return F4 ? static_cast<uint32_t>(j & 1) * 2 : j; }
-};
-
 // ---- activation ----
 // Two fp32 values in one 64-bit register: Blackwell's packed multiply and fused multiply-add.
 __device__ __forceinline__ uint64_t pack_f2(float a, float b) {
@@ -200,30 +188,6 @@ __device__ __forceinline__ void apply_act(float (&v)[N], int act) {
 // in 185 us in mxfp8 (3.0 PFLOP/s, 78 %); 25664 x 384 x 1536 with fp32 outputs in 35 us (4.5 TB/s written), 44 with GELU.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kPairThreads = 18 * 32;
-
-template <bool F4, int BN>
-struct PairCfg {
-  // Rows of the staging tiles: 128 bytes, or 64 where the room is better used for a stage more (BN 256: 8192 x 4096 x 8192
-  // in mxfp8 in 185 us with five stages, in 193 with four and 128-byte rows).
-  static constexpr int kRow = BN == 256 ? 64 : 128;
-  static constexpr int kStages = BN == 256 ? 5 : 6;
-  static constexpr uint32_t kA = 128 * 128, kW = BN / 2 * 128;
-  static constexpr uint32_t kSfa = 512 * Elem<F4>::kKt, kSfw = BN / 128 * kSfa;
-  static constexpr uint32_t kOffSf = kA + kW;
-  static constexpr uint32_t kStage = (kOffSf + kSfa + kSfw + 1023) / 1024 * 1024;
-  static constexpr uint32_t kTx = 2 * (kA + Elem<F4>::kTxW * BN / 256 + kSfa + kSfw);  // both CTAs
-  static constexpr uint32_t kOffStaging = kStages * kStage;
-  static constexpr uint32_t kStaging = 32 * kRow;  // 32 rows for each epilogue warp
-  static constexpr uint32_t kOffBias = kOffStaging + 16 * kStaging;  // 64 columns for each epilogue warp
-  static constexpr uint32_t kOffBars = kOffBias + 16 * 64 * 4;
-  static constexpr uint32_t kSmem = 1024 + kOffBars + 256;
-  static constexpr int kAccs = BN == 256 ? 2 : 3;                // accumulators, 128 columns apart
-  static constexpr uint32_t kSfwCols = 4 * (BN / 128);
-  static constexpr uint32_t kColSf = 384, kSfCols = (4 + kSfwCols) * Elem<F4>::kKt;  // a slot
-  static_assert(BN == 128 || BN == 256, "tile width");
-  static_assert(kColSf + kStages * kSfCols <= 512, "tensor memory");
-  static_assert((2 * kStages + 2 * kAccs + 2) * 8 + 16 <= 256, "barrier area");
-};
 
 struct PairArgs {
   const float* bias;
@@ -535,24 +499,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 constexpr int kSliceThreads = 128;   // without the quantising warps
 constexpr int kFuseGroups = 4, kFuseThreads = 64 + 64 * kFuseGroups;
 constexpr int kFuseRows = KO_MXFP4_FUSED_ROWS;
-
-template <bool F4, int BN>
-struct SliceCfg {
-  static constexpr uint32_t kW = 128 * 128, kX = BN * 128, kSf = 512 * Elem<F4>::kKt;
-  static constexpr uint32_t kOffSf = kW + kX;
-  static constexpr uint32_t kStage = (kW + kX + 2 * kSf + 1023) / 1024 * 1024;
-  static constexpr uint32_t kTx = Elem<F4>::kTxW + kX + 2 * kSf;
-  static constexpr int kStages = BN <= 32 ? 5 : BN <= 64 ? 4 : 3;  // about 100 KB: two CTAs share an SM
-  static constexpr uint32_t kOffBars = kStages * kStage;
-  static constexpr uint32_t kSmem = 1024 + kOffBars + 256;
-  static constexpr uint32_t kAccCols = BN < 32 ? 32 : BN;
-  static constexpr uint32_t kSfCols = 8 * Elem<F4>::kKt;
-  static constexpr uint32_t kNeed = kAccCols + kStages * kSfCols;
-  static constexpr uint32_t kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
-  static_assert(kNeed <= 256, "two CTAs of an SM share 512 columns");
-  static_assert(BN * 128 * 4 <= kOffBars, "partial sums reuse the stages");
-  static_assert((2 * kStages + 1) * 8 + 16 <= 256, "barrier area");
-};
 
 struct SliceArgs {
   const float* bias;
