@@ -333,8 +333,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       mma_commit_pair_w(mma_done);
     }
-    volatile int never = 0;
-    if (!mbar_wait_warp(mma_done, 0, &never)) *abort_flag = 1;
   } else {
     const int e = warp - 2, q = warp & 3;
     const int set = e >> 3;      // BN 256: the shared half of every tile or the other one; BN 128: even or odd tiles
@@ -471,13 +469,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  // After an abort loads may be in flight that no MMA waited for. They land within microseconds, and their barrier may be
-  // the peer's, so this CTA gives them ten milliseconds before it leaves.
-  if (threadIdx.x == 0 && *abort_flag) {
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < 10000000ull) {}
+  // Also after an abort, what was issued completes before its memory is given back. The wait comes after the CTA's other roles
+  // have ended, whose waits cover a tile each: begun at the start, it would put its limit on the whole product. After an abort
+  // loads may be in flight that no MMA waited for, too. They land within microseconds, and their barrier may be the peer's, so
+  // this CTA gives them ten milliseconds before it leaves.
+  if (warp == 1) {
+    volatile int never = 0;
+    if (!mbar_wait_warp(mma_done, 0, &never)) *abort_flag = 1;
+    if (*abort_flag) {
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 10000000ull) {}
+    }
+    __syncwarp();
   }
-  __syncthreads();
   cluster_sync();  // neither CTA leaves while the other's arrivals, copies or MMAs may still reach it
   if (warp == 1) {
     tc_fence_after();
