@@ -402,10 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tf32x3_kernel(const __g
         mma_commit_pair_w(&o_full[g & 1]);
       }
     }
-    // Drain: every MMA the leader issued completes before either CTA releases its tensor memory.
-    if (rank == 0) mma_commit_pair_w(mma_done);
-    volatile int never = 0;
-    if (!warp_wait(mma_done, 0, &never)) *abort_flag = 1;
+    if (rank == 0) mma_commit_pair_w(mma_done);  // for the drain below
   } else if (warp < kLoadWarp0) {
     // ---------------- softmax + output, one thread per query row ----------------
     // Block g (key block j of item g / nkb), two passes over S_g in tensor memory: the first finds the row
@@ -669,10 +666,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tf32x3_kernel(const __g
   }
 
   // Neither CTA leaves while the other may still arrive on its barriers or (the leader's MMAs) read its shared and
-  // tensor memory: every MMA is complete (mma_done, waited by warp 0 of each CTA above) and every thread of the
-  // pair is past its last arrival.
+  // tensor memory: every MMA is complete (mma_done, waited by warp 0 of each CTA) and every thread of the pair is past
+  // its last arrival. The wait comes after the CTA's other roles have ended, whose waits cover a block of keys each:
+  // begun at the start by the CTA that issues no MMAs, it would put its limit on the whole launch.
   tc_fence_before();
   __syncthreads();
+  if (warp == 0) {
+    volatile int never = 0;
+    if (!warp_wait(mma_done, 0, &never)) *abort_flag = 1;
+  }
   cluster_sync();
   if (warp == 0) {
     tc_fence_after();

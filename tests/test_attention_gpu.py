@@ -73,3 +73,20 @@ def test_attention_writes_into_out_and_rejects_bad_shapes(cuda):
         K.attention(q, k, v, 1, 0.125)          # head_dim 128
     with pytest.raises(ValueError):
         K.attention(q.cpu(), k, v, 2, 0.125)    # no CPU path
+
+
+def test_launch_longer_than_a_wait(cuda):
+    """1.1e15 operations, about four seconds: every wait of the kernel has a limit of two, and each covers a block of keys,
+    not the launch. The batch items are one, so that their results are too."""
+    n, heads, hd, batch = 1 << 17, 16, 64, 16
+    g = torch.Generator(device=cuda).manual_seed(5)
+    q, k, v = (torch.randn((1, n, heads * hd), generator=g, device=cuda) for _ in range(3))
+    one = K.attention(q, k, v, heads, hd ** -0.5)
+    K.check_device_status(cuda)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    out = K.attention(*(t.expand(batch, -1, -1) for t in (q, k, v)), heads, hd ** -0.5)
+    end.record()
+    K.check_device_status(cuda)
+    assert start.elapsed_time(end) > 2000, "the launch is too short to show anything"
+    assert all(torch.equal(out[b], one[0]) for b in range(batch))
