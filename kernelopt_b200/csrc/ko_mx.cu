@@ -409,6 +409,7 @@ extern "C" int ko_quantize_mx(const void* x, int dtype, int64_t rows, int64_t K,
   const std::string who = "ko_quantize_mx: ";
   if (rows < 0 || rows > kMaxRows || K < 1 || K > kMaxK || ldx < K)
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "need 0 <= rows <= 2^31, 1 <= K <= 2^24 and ldx >= K");
+  if (!extent_ok(rows, ldx)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "the rows' pitch spans more than 2^46 elements");
   if (!dtype_ok(dtype) || !fmt_ok(fmt)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "unknown element type or format");
   if (rows == 0) return KO_OK;
   if (!x || !codes || !scales) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
@@ -478,6 +479,8 @@ extern "C" int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, in
   const std::string who = "ko_residual_rmsnorm: ";
   if (rows < 0 || rows > kMaxRows || C < 1 || C > 32768 || ldh < C || (o && ldo < C))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "need 0 <= rows <= 2^31, 1 <= C <= 32768 and pitches of at least C");
+  if (!extent_ok(rows, ldh) || (o && !extent_ok(rows, ldo)))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "the rows' pitch spans more than 2^46 elements");
   if (!dtype_ok(dtype)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "unknown element type");
   if (!(eps >= 0.f)) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "eps must not be negative");
   if (y ? (codes || scales) : (!codes || !scales || !fmt_ok(fmt)))

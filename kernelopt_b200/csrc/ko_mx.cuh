@@ -25,9 +25,12 @@ inline bool groups_of_8(const void* p, int dtype, int64_t pitch, int64_t width) 
   const int64_t group = 8 * dtype_size(dtype);
   return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(group) == 0 && pitch % 8 == 0 && width % 8 == 0;
 }
-// Bounds that keep every size and offset product of these entry points inside 62 bits.
+// Bounds of the entry points: rows times K is at most 2^55, and what rows and their pitch span (extent_ok) 2^46 elements, more
+// than an address space holds, so that every size, offset and end address in bytes stays inside 62 bits.
 constexpr int64_t kMaxRows = int64_t(1) << 31;
 constexpr int64_t kMaxK = int64_t(1) << 24;
+constexpr int64_t kMaxExtent = int64_t(1) << 46;
+inline bool extent_ok(int64_t rows, int64_t pitch) { return rows <= 1 || pitch <= kMaxExtent / rows; }
 
 #if defined(__CUDACC__)
 

@@ -850,7 +850,6 @@ int launch_pair(const Call& c) {
   using E = Elem<F4>;
   constexpr const char* who = "ko_linear_mxfp4";
   const int64_t mt = (c.M + 255) / 256, nt = (c.N + BN - 1) / BN;
-  if (mt * nt > INT32_MAX / 16) return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(who) + ": too many output tiles");
   CUtensorMap ma, mw, msa, msw, mo;
   const int64_t es = static_cast<int64_t>(sizeof(T));
   const bool tma_out = ko::aligned16(c.out) && c.N * es % 16 == 0;
@@ -905,7 +904,6 @@ int launch_slice(const Call& c) {
   using E = Elem<F4>;
   constexpr const char* who = "ko_linear_mxfp4";
   const int64_t mt = (c.M + BN - 1) / BN, nt = (c.N + 127) / 128;
-  if (mt * nt > INT32_MAX / 16) return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(who) + ": too many output tiles");
   CUtensorMap mx, mw, msx, msw;
   int rc = encode_codes(&mw, c.wc, KO_MXFP4, !F4, c.N, c.Kp, 128, who);
   if (!rc) rc = encode_scales(&msw, c.ws, c.N, c.Kp, E::kKt, 1, who);
@@ -986,6 +984,9 @@ int check_linear(const char* name, int64_t M, int64_t K, int64_t N, int act, con
   auto bad = [&](const char* what) { return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
   if (M < 0 || M > kMaxRows || K < 1 || K > kMaxK || N < 1 || N > kMaxRows)
     return bad("need 0 <= M <= 2^31, 1 <= K <= 2^24 and 1 <= N <= 2^31");
+  // Tiles are counted in 32 bits, with room for a band of eight or a cluster of eight slices. Checked here, before anything
+  // is launched; it holds M * N to 2^42.
+  if (((M + 255) / 256) * ((N + 127) / 128) > INT32_MAX / 16) return bad("too many output tiles");
   if (!dtype_ok(out_dtype)) return bad("unknown output type");
   if (act != KO_ACT_NONE && act != KO_ACT_GELU && act != KO_ACT_RELU)
     return bad("act must be KO_ACT_NONE, KO_ACT_GELU or KO_ACT_RELU");
@@ -1042,6 +1043,7 @@ extern "C" int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx,
   auto bad = [&](const char* what) { return ko::fail(KO_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
   if (!dtype_ok(x_dtype)) return bad("unknown element type");
   if (ldx < K) return bad("ldx must be at least K");
+  if (!extent_ok(M, ldx)) return bad("the rows' pitch spans more than 2^46 elements");
   if (M == 0) return KO_OK;
   if (!x || reinterpret_cast<uintptr_t>(x) % static_cast<uintptr_t>(dtype_size(x_dtype)) != 0)
     return bad("x must be given, aligned to its elements");

@@ -165,3 +165,23 @@ def test_oracle_against_hand_computed_blocks():
     assert q[0, :4].tolist() == [448, 448, 1.0, 2.0 ** -9]    # saturated; 1.0625 is a tie and goes to the even 1
     v[0, 1] = np.inf
     assert np.isnan(OM.round_trip(v, "mxfp8")[0, :32]).all() and np.isfinite(OM.round_trip(v, "mxfp8")[0, 32:]).all()
+
+
+BIG = 1 << 31
+HUGE = 1 << 60  # a pitch whose product with the rows leaves 64 bits
+
+
+@pytest.mark.parametrize("name,args,why", [
+    ("ko_quantize_mx", (A, 0, 16, 64, HUGE, 0, A, A, None), "pitch"),
+    ("ko_residual_rmsnorm", (A, HUGE, A, 64, None, None, A, 0, 1e-6, 16, 64, A, A, 0, None, None, None), "pitch"),
+    ("ko_residual_rmsnorm", (A, 64, A, HUGE, None, None, A, 0, 1e-6, 16, 64, A, A, 0, None, None, None), "pitch"),
+    ("ko_linear_quantize_mxfp4", (A, 0, HUGE, A, A, None, 16, 64, 64, 0, A, 0, None, 0, None, None), "pitch"),
+    ("ko_linear_quantize_mxfp4", (A, 0, 64, A, A, None, BIG, 64, BIG, 0, A, 0, A, HUGE, None, None), "tiles"),
+    ("ko_linear_mxfp4", (A, A, 0, A, A, None, BIG, 64, BIG, 0, A, 0, None, None), "tiles"),
+    ("ko_linear_mxfp4", (A, A, 1, A, A, None, 1 << 30, 64, 1 << 13, 0, A, 0, None, None), "tiles"),
+])
+def test_sizes_whose_products_leave_the_range_are_refused(name, args, why):
+    """Before their extents are compared with anything, and before anything is launched: there is no device here to refuse
+    a launch with another reason."""
+    with pytest.raises(ValueError, match=why):
+        _lib.call(name, *args)
