@@ -328,10 +328,10 @@ int ko_pack_weight_mxfp4(const void* w, int dtype, int64_t K, int64_t N, void* c
 
 /* v = h + (o + bias) * scale;  y = v / sqrt(mean(v^2) + eps) * gamma over rows of C (statistics and y in fp32 from the
  * unrounded v). h, o: [rows][C] of `dtype`, rows ldh / ldo elements apart; bias, scale, gamma: [C] of `dtype`; o NULL
- * = no residual (bias and scale then unused), bias / scale NULL = 0 / 1. h_out: [rows][C] receives v rounded to
- * `dtype`, or NULL; it may be h or o itself where that is contiguous, and overlaps them in no other way. Exactly one form of y: y [rows][C] of `dtype`, or y NULL and
- * codes, scales in `fmt`. 1 <= C <= 32768. Stands beside ko_residual_layernorm for models that normalise by the root
- * mean square. */
+ * = no residual (bias and scale then NULL too), bias / scale NULL = 0 / 1. h_out: [rows][C] receives v rounded to
+ * `dtype`, or NULL. Exactly one form of y: y [rows][C] of `dtype`, or y NULL and codes, scales in `fmt`. h_out or y may be
+ * h or o itself where that is contiguous; an output that overlaps an input in another way, or another output, is refused.
+ * 1 <= C <= 32768. Stands beside ko_residual_layernorm for models that normalise by the root mean square. */
 int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, int64_t ldo, const void* bias, const void* scale,
                         const void* gamma, int dtype, float eps, int64_t rows, int64_t C, void* h_out, void* y, int fmt,
                         void* codes, void* scales, ko_stream_t stream);

@@ -18,6 +18,11 @@ void set_error(const std::string& msg);
 int fail(int code, const std::string& msg);            // records msg, returns code
 int check_launch(const char* what);                    // cudaGetLastError() -> status
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Whether n bytes at p and m bytes at q share one. A null pointer or an empty range shares none.
+inline bool ranges_meet(const void* p, int64_t n, const void* q, int64_t m) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return p && q && n > 0 && m > 0 && a < b + static_cast<uintptr_t>(m) && b < a + static_cast<uintptr_t>(n);
+}
 
 // Device properties cached per device (SM count, opt-in shared memory).
 struct DeviceInfo {

@@ -490,16 +490,30 @@ extern "C" int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, in
   if (!h || !gamma) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
   if (!o && (bias || scale))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "bias and scale belong to o");
-  // A row is read whole before it is written, by the threads that write it: in place is fine, any other overlap is not.
-  const int64_t elem = dtype_size(dtype);
-  auto meets = [&](const void* a, int64_t lda) {
-    const char *a0 = static_cast<const char*>(a), *b0 = static_cast<const char*>(h_out);
-    const bool apart = !a || !h_out || a0 + ((rows - 1) * lda + C) * elem <= b0 || b0 + rows * C * elem <= a0;
-    return !apart && !(a0 == b0 && (lda == C || rows == 1));
+  // A row of h and o is read whole before it is written, by the threads that write it: h_out or y in place of one of them is
+  // fine. Every other overlap of an output is not: with another row, with the vectors, that all rows read, or with another
+  // output.
+  const int64_t es = dtype_size(dtype), out_bytes = rows * C * es;
+  struct Range {
+    const void* p;
+    int64_t bytes, pitch;
   };
-  if (meets(h, ldh) || meets(o, ldo))
-    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "h_out overlaps h or o other than in place (the same contiguous rows)");
-  const int64_t es = dtype_size(dtype);
+  const Range ins[] = {{h, ((rows - 1) * ldh + C) * es, ldh}, {o, ((rows - 1) * ldo + C) * es, ldo}};
+  const Range outs[] = {{h_out, out_bytes, C}, {y, out_bytes, C}, {codes, y ? 0 : ko_mx_codes_bytes(rows, C, fmt), 0},
+                        {scales, y ? 0 : ko_mx_scales_bytes(rows, C), 0}};
+  for (int i = 0; i < 4; ++i) {
+    const Range& out = outs[i];
+    bool meets = false;
+    for (const Range& in : ins) {
+      const bool in_place = in.p == out.p && (in.pitch == out.pitch || (rows == 1 && out.pitch == C));
+      meets = meets || (!in_place && ko::ranges_meet(out.p, out.bytes, in.p, in.bytes));
+    }
+    for (const void* v : {bias, scale, gamma}) meets = meets || ko::ranges_meet(out.p, out.bytes, v, C * es);
+    for (int j = 0; j < i; ++j) meets = meets || ko::ranges_meet(out.p, out.bytes, outs[j].p, outs[j].bytes);
+    if (meets)
+      return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "an output overlaps an input or another output (h_out or y may be h or o "
+                                                     "itself, the same contiguous rows)");
+  }
   bool vec = ldh % 8 == 0 && (!o || ldo % 8 == 0);
   const void* elems[] = {h, o, bias, scale, gamma, h_out, y};
   for (const void* p : elems) {

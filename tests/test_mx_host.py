@@ -185,3 +185,40 @@ def test_sizes_whose_products_leave_the_range_are_refused(name, args, why):
     a launch with another reason."""
     with pytest.raises(ValueError, match=why):
         _lib.call(name, *args)
+
+
+def norm_call(h=A, ldh=64, o=9 * A, ldo=64, bias=None, scale=None, gamma=20 * A, rows=4, c=64, h_out=11 * A, y=13 * A, fmt=0,
+              codes=None, scales=None):
+    return (h, ldh, o, ldo, bias, scale, gamma, 0, 1e-6, rows, c, h_out, y, fmt, codes, scales, None)
+
+
+ROW = 64 * 4          # bytes of a row of the calls below
+
+
+@pytest.mark.parametrize("args", [
+    norm_call(y=A + ROW), norm_call(y=A - ROW), norm_call(y=9 * A + ROW), norm_call(y=A + 4),      # shifted over h or o
+    norm_call(ldh=72, y=A), norm_call(o=A, ldo=72, h_out=None, y=A),                               # in place of strided rows
+    norm_call(y=11 * A), norm_call(y=11 * A + 3 * ROW), norm_call(h_out=A, y=A),                   # over h_out
+    norm_call(h_out=20 * A), norm_call(y=20 * A - 4 * ROW + 4), norm_call(bias=13 * A + 64),       # over gamma and bias
+    norm_call(scale=11 * A + 4 * ROW - 16),
+    norm_call(y=None, codes=A + 512, scales=14 * A), norm_call(y=None, codes=14 * A, scales=9 * A + 16),   # over h, o
+    norm_call(y=None, codes=11 * A + 992, scales=14 * A), norm_call(y=None, codes=14 * A, scales=11 * A),  # over h_out
+    norm_call(y=None, codes=14 * A, scales=14 * A), norm_call(y=None, fmt=1, codes=14 * A, scales=14 * A + 496),
+    norm_call(y=None, codes=20 * A + 240, scales=14 * A),
+])
+def test_norm_outputs_that_overlap_are_refused(args):
+    with pytest.raises(ValueError, match="overlaps"):
+        _lib.call("ko_residual_rmsnorm", *args)
+
+
+@pytest.mark.parametrize("args", [
+    norm_call(), norm_call(y=A), norm_call(y=9 * A), norm_call(h_out=A, y=9 * A), norm_call(h_out=9 * A, y=A),
+    norm_call(o=A, h_out=None, y=A), norm_call(rows=1, ldh=72, y=A), norm_call(o=None, ldo=0, h_out=None, y=A),
+    norm_call(y=A + 4 * ROW), norm_call(y=A - 4 * ROW), norm_call(y=11 * A + 4 * ROW),
+    norm_call(y=None, codes=14 * A, scales=14 * A + 256), norm_call(y=None, fmt=1, codes=A + 4 * ROW, scales=A + 4 * ROW + 512),
+])
+def test_norm_outputs_in_place_or_apart_pass_the_checks(args):
+    if torch.cuda.is_available():
+        pytest.skip("would launch on made-up addresses")
+    with pytest.raises(_lib.KernelError):
+        _lib.call("ko_residual_rmsnorm", *args)

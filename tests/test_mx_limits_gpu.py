@@ -1,4 +1,5 @@
-"""The microscaled operators at the ends of what they take: products that run longer than any one wait of their kernels may."""
+"""The microscaled operators at the ends of what they take: products that run longer than any one wait of their kernels may,
+and norms whose outputs take the place of their inputs."""
 from __future__ import annotations
 
 import pytest
@@ -40,3 +41,19 @@ def test_product_longer_than_a_wait(cuda):
     assert start.elapsed_time(end) > 2000, "the product is too short to show anything"
     for r in range(0, m, 4096):
         assert bool((out[r:r + 4096].view(16, 256, n // 256, 256) == want[None, :, None, :]).all()), r
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float32, _lib.KO_F32), (torch.bfloat16, _lib.KO_BF16)])
+@pytest.mark.parametrize("rows,c", [(1, 33), (5, 384), (130, 1000), (7, 4096), (3, 16392), (3, 32768)])
+def test_norm_output_in_place(cuda, rows, c, dtype, code):
+    """y in the place of h or of o, and v in the other's."""
+    g = torch.Generator(device=cuda).manual_seed(rows + c)
+    h, o = (torch.randn((rows, c), generator=g, device=cuda).to(dtype) for _ in range(2))
+    gamma = (1 + 0.1 * torch.randn(c, generator=g, device=cuda)).to(dtype)
+    v, y = K.residual_rmsnorm(h, o, None, None, gamma, 1e-6)
+    for swap in (False, True):
+        a, b = h.clone(), o.clone()
+        v_at, y_at = (b, a) if swap else (a, b)
+        _lib.call("ko_residual_rmsnorm", a.data_ptr(), c, b.data_ptr(), c, None, None, gamma.data_ptr(), code, 1e-6, rows, c,
+                  v_at.data_ptr(), y_at.data_ptr(), 0, None, None, torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(v_at, v) and torch.equal(y_at, y)
