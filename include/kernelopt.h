@@ -309,7 +309,8 @@ int ko_box_head_f32(const float* x, const float* w, const float* bias, const flo
  * Element k of a row stands for code * 2^(byte - 127). A block's byte is floor(log2(max |v|)) - emax + 127, held to 0
  * or above, with emax 2 (MXFP4) or 8 (MXFP8); its codes are v / 2^(byte - 127) to nearest even, saturating at the
  * largest element. A block that holds a NaN or an infinity gets byte 255 (NaN) and zero codes. Both buffers are 16-byte
- * aligned. The reference has no reduced-precision path: no counterpart there. */
+ * aligned. No output of these entry points may overlap an input, a workspace or another output, but for what
+ * ko_residual_rmsnorm says; such calls are refused. The reference has no reduced-precision path: no counterpart there. */
 int64_t ko_mx_codes_bytes(int64_t rows, int64_t K, int fmt); /* -1 for a bad size or format */
 int64_t ko_mx_scales_bytes(int64_t rows, int64_t K);         /* -1 for a bad size */
 
@@ -348,8 +349,7 @@ int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_fmt, const 
  * KO_MXFP4 and multiplied, with the result of ko_quantize_mx and ko_linear_mxfp4 bit for bit. Up to KO_MXFP4_FUSED_ROWS
  * rows, the tokens of a decoding step, are quantised inside the product's kernel: a launch of their own and the round trip
  * through memory would cost more, and `workspace` may be NULL. More rows go through `workspace`: 16-byte aligned,
- * ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes (0 up to KO_MXFP4_FUSED_ROWS rows, -1 for a bad size). out must not
- * overlap x. */
+ * ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes (0 up to KO_MXFP4_FUSED_ROWS rows, -1 for a bad size). */
 #define KO_MXFP4_FUSED_ROWS 16
 int64_t ko_linear_quantize_mxfp4_workspace_bytes(int64_t M, int64_t K);
 int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx, const void* w_codes, const void* w_scales,

@@ -416,6 +416,10 @@ extern "C" int ko_quantize_mx(const void* x, int dtype, int64_t rows, int64_t K,
   const int64_t es = dtype_size(dtype);
   if (!aligned_to(x, es) || !ko::aligned16(codes) || !ko::aligned16(scales))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "x must be aligned to its elements, codes and scales to 16 bytes");
+  const Range in = span_of(x, rows, ldx, K, es), c = {codes, ko_mx_codes_bytes(rows, K, fmt)},
+              sc = {scales, ko_mx_scales_bytes(rows, K)};
+  if (meets(c, {in, sc}) || meets(sc, {in}))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "codes or scales overlap x or each other");
   const bool vec = groups_of_8(x, dtype, ldx, K);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool f4 = fmt == KO_MXFP4;
@@ -439,6 +443,9 @@ extern "C" int ko_dequantize_mx(const void* codes, const void* scales, int fmt, 
   if (!codes || !scales || !out) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
   if (!ko::aligned16(codes) || !ko::aligned16(scales) || !aligned_to(out, dtype_size(dtype)))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "codes and scales must be 16-byte aligned, out to its elements");
+  if (meets({out, rows * K * dtype_size(dtype)},
+            {{codes, ko_mx_codes_bytes(rows, K, fmt)}, {scales, ko_mx_scales_bytes(rows, K)}}))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "out overlaps codes or scales");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == KO_F32) return launch_dequantize<float>(codes, scales, fmt, rows, K, out, s);
   if (dtype == KO_BF16) return launch_dequantize<__nv_bfloat16>(codes, scales, fmt, rows, K, out, s);
@@ -454,6 +461,10 @@ extern "C" int ko_pack_weight_mxfp4(const void* w, int dtype, int64_t K, int64_t
   if (!w || !codes || !scales) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "null pointer");
   if (!aligned_to(w, dtype_size(dtype)) || !ko::aligned16(codes) || !ko::aligned16(scales))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "w must be aligned to its elements, codes and scales to 16 bytes");
+  const Range in = {w, K * N * dtype_size(dtype)}, out = {codes, ko_mx_codes_bytes(N, K, KO_MXFP4)},
+              tiles = {scales, ko_mx_scales_bytes(N, K)};
+  if (meets(out, {in, tiles}) || meets(tiles, {in}))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "codes or scales overlap w or each other");
   const int64_t kblocks = padded_k(K) / 32, n_rows = (N + 127) / 128 * 128;
   const int64_t blocks = kblocks * ((n_rows + kThreads - 1) / kThreads);
   if (blocks > 0x7fffffff) return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "the weight is too large");
@@ -494,26 +505,18 @@ extern "C" int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, in
   // fine. Every other overlap of an output is not: with another row, with the vectors, that all rows read, or with another
   // output.
   const int64_t es = dtype_size(dtype), out_bytes = rows * C * es;
-  struct Range {
-    const void* p;
-    int64_t bytes, pitch;
+  const Range hs = span_of(h, rows, ldh, C, es), os = span_of(o, rows, ldo, C, es);
+  const Range vs[] = {{bias, C * es}, {scale, C * es}, {gamma, C * es}};
+  const Range ho = {h_out, out_bytes}, yo = {y, out_bytes}, co = {codes, y ? 0 : ko_mx_codes_bytes(rows, C, fmt)},
+              so = {scales, y ? 0 : ko_mx_scales_bytes(rows, C)};
+  auto meets_rows = [&](const Range& out, const Range& in, int64_t pitch) {
+    return !(in.p == out.p && (rows == 1 || pitch == C)) && meets(out, {in});
   };
-  const Range ins[] = {{h, ((rows - 1) * ldh + C) * es, ldh}, {o, ((rows - 1) * ldo + C) * es, ldo}};
-  const Range outs[] = {{h_out, out_bytes, C}, {y, out_bytes, C}, {codes, y ? 0 : ko_mx_codes_bytes(rows, C, fmt), 0},
-                        {scales, y ? 0 : ko_mx_scales_bytes(rows, C), 0}};
-  for (int i = 0; i < 4; ++i) {
-    const Range& out = outs[i];
-    bool meets = false;
-    for (const Range& in : ins) {
-      const bool in_place = in.p == out.p && (in.pitch == out.pitch || (rows == 1 && out.pitch == C));
-      meets = meets || (!in_place && ko::ranges_meet(out.p, out.bytes, in.p, in.bytes));
-    }
-    for (const void* v : {bias, scale, gamma}) meets = meets || ko::ranges_meet(out.p, out.bytes, v, C * es);
-    for (int j = 0; j < i; ++j) meets = meets || ko::ranges_meet(out.p, out.bytes, outs[j].p, outs[j].bytes);
-    if (meets)
-      return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "an output overlaps an input or another output (h_out or y may be h or o "
-                                                     "itself, the same contiguous rows)");
-  }
+  if (meets_rows(ho, hs, ldh) || meets_rows(ho, os, ldo) || meets_rows(yo, hs, ldh) || meets_rows(yo, os, ldo) ||
+      meets(co, {hs, os, so, vs[0], vs[1], vs[2]}) || meets(so, {hs, os, vs[0], vs[1], vs[2]}) ||
+      meets(ho, {yo, co, so, vs[0], vs[1], vs[2]}) || meets(yo, {vs[0], vs[1], vs[2]}))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, who + "an output overlaps an input or another output (h_out or y may be h or o "
+                                                   "itself, the same contiguous rows)");
   bool vec = ldh % 8 == 0 && (!o || ldo % 8 == 0);
   const void* elems[] = {h, o, bias, scale, gamma, h_out, y};
   for (const void* p : elems) {

@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "ko_common.cuh"
 
 namespace komx {
@@ -31,6 +33,19 @@ constexpr int64_t kMaxRows = int64_t(1) << 31;
 constexpr int64_t kMaxK = int64_t(1) << 24;
 constexpr int64_t kMaxExtent = int64_t(1) << 46;
 inline bool extent_ok(int64_t rows, int64_t pitch) { return rows <= 1 || pitch <= kMaxExtent / rows; }
+// What an output may not share a byte with: the threads that write it are not those that read the others.
+struct Range {
+  const void* p;
+  int64_t bytes;
+};
+inline Range span_of(const void* p, int64_t rows, int64_t pitch, int64_t width, int64_t size) {
+  return {p, ((rows - 1) * pitch + width) * size};
+}
+inline bool meets(const Range& out, std::initializer_list<Range> others) {
+  for (const Range& r : others)
+    if (ko::ranges_meet(out.p, out.bytes, r.p, r.bytes)) return true;
+  return false;
+}
 
 #if defined(__CUDACC__)
 

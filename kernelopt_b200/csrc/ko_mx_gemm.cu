@@ -1000,6 +1000,14 @@ int check_linear(const char* name, int64_t M, int64_t K, int64_t N, int act, con
   return KO_OK;
 }
 
+// The weight and the bias as what an output may not overlap.
+struct Operands {
+  Range codes, scales, bias;
+};
+Operands operands(const void* w_codes, const void* w_scales, const float* bias, int64_t K, int64_t N) {
+  return {{w_codes, ko_mx_codes_bytes(N, K, KO_MXFP4)}, {w_scales, ko_mx_scales_bytes(N, K)}, {bias, 4 * N}};
+}
+
 // ko_linear_mxfp4 after the checks of its operands.
 int product(Call c, int a_fmt, int out_dtype, const char* name) {
   const int rc = ko::device_or_fail(&c.info, name);
@@ -1022,6 +1030,10 @@ extern "C" int ko_linear_mxfp4(const void* a_codes, const void* a_scales, int a_
   if (M == 0) return KO_OK;
   if (!a_codes || !a_scales || !ko::aligned16(a_codes) || !ko::aligned16(a_scales))
     return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_linear_mxfp4: codes and scales must be given, 16-byte aligned");
+  const Operands w = operands(w_codes, w_scales, bias, K, N);
+  if (meets({out, M * N * dtype_size(out_dtype)}, {{a_codes, ko_mx_codes_bytes(M, K, a_fmt)},
+                                                  {a_scales, ko_mx_scales_bytes(M, K)}, w.codes, w.scales, w.bias}))
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, "ko_linear_mxfp4: out overlaps an operand");
   return product(Call{a_codes, a_scales, w_codes, w_scales, bias, M, K, N, padded_k(K), act, out, dev_status,
                       reinterpret_cast<cudaStream_t>(stream), nullptr, nullptr, 0, false},
                  a_fmt, out_dtype, name);
@@ -1047,12 +1059,14 @@ extern "C" int ko_linear_quantize_mxfp4(const void* x, int x_dtype, int64_t ldx,
   if (M == 0) return KO_OK;
   if (!x || reinterpret_cast<uintptr_t>(x) % static_cast<uintptr_t>(dtype_size(x_dtype)) != 0)
     return bad("x must be given, aligned to its elements");
-  const char *x0 = static_cast<const char*>(x), *out0 = static_cast<const char*>(out);
-  if (x0 < out0 + M * N * dtype_size(out_dtype) && out0 < x0 + ((M - 1) * ldx + K) * dtype_size(x_dtype))
-    return bad("out overlaps x");
+  const Operands w = operands(w_codes, w_scales, bias, K, N);
+  const Range in = span_of(x, M, ldx, K, dtype_size(x_dtype)), to = {out, M * N * dtype_size(out_dtype)};
+  if (meets(to, {in, w.codes, w.scales, w.bias})) return bad("out overlaps x, the weight or the bias");
   if (M > kFuseRows) {
     if (!workspace || !ko::aligned16(workspace) || workspace_bytes < ko_linear_quantize_mxfp4_workspace_bytes(M, K))
       return bad("the workspace must be 16-byte aligned and hold ko_linear_quantize_mxfp4_workspace_bytes(M, K) bytes");
+    if (meets({workspace, ko_linear_quantize_mxfp4_workspace_bytes(M, K)}, {in, to, w.codes, w.scales, w.bias}))
+      return bad("the workspace overlaps x, out, the weight or the bias");
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     uint8_t* scales = codes + (ko_mx_codes_bytes(M, K, KO_MXFP4) + 15) / 16 * 16;
     rc = ko_quantize_mx(x, x_dtype, M, K, ldx, KO_MXFP4, codes, scales, stream);

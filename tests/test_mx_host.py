@@ -222,3 +222,50 @@ def test_norm_outputs_in_place_or_apart_pass_the_checks(args):
         pytest.skip("would launch on made-up addresses")
     with pytest.raises(_lib.KernelError):
         _lib.call("ko_residual_rmsnorm", *args)
+
+
+def at(i):
+    return 16 * A + i * 64 * A      # far from each other, for the small operands below
+
+
+# x or w 64 x 64 float32 (16384 bytes), its codes 64 x 64 bytes (mxfp4; Kp 128), scales 512 bytes; out 64 x 64 float32
+@pytest.mark.parametrize("name,args", [
+    ("ko_quantize_mx", (at(0), 0, 64, 64, 64, 0, at(0) + 16368, at(1), None)),                  # codes over x
+    ("ko_quantize_mx", (at(0), 0, 64, 64, 64, 0, at(1), at(0) - 496, None)),                    # scales over x
+    ("ko_quantize_mx", (at(0), 0, 64, 64, 64, 0, at(1), at(1) + 4080, None)),                   # scales over codes
+    ("ko_quantize_mx", (at(0), 0, 64, 64, 128, 1, at(0) + 32256 - 16, at(1), None)),            # codes over strided x's end
+    ("ko_dequantize_mx", (at(0), at(1), 0, 64, 64, at(0) + 4092, 0, None)),                     # out over codes
+    ("ko_dequantize_mx", (at(0), at(1), 0, 64, 64, at(1) + 508, 0, None)),                      # out over scales
+    ("ko_pack_weight_mxfp4", (at(0), 0, 64, 64, at(0) - 4080, at(1), None)),                    # codes over w
+    ("ko_pack_weight_mxfp4", (at(0), 0, 64, 64, at(1), at(0) + 16368, None)),                   # scales over w
+    ("ko_pack_weight_mxfp4", (at(0), 0, 64, 64, at(1), at(1), None)),                           # scales over codes
+    ("ko_linear_mxfp4", (at(0), at(1), 0, at(2), at(3), at(4), 64, 64, 64, 0, at(0) + 4092, 0, None, None)),   # a's codes
+    ("ko_linear_mxfp4", (at(0), at(1), 1, at(2), at(3), at(4), 64, 64, 64, 0, at(0) + 8188, 0, None, None)),
+    ("ko_linear_mxfp4", (at(0), at(1), 0, at(2), at(3), at(4), 64, 64, 64, 0, at(1) + 508, 0, None, None)),    # a's scales
+    ("ko_linear_mxfp4", (at(0), at(1), 0, at(2), at(3), at(4), 64, 64, 64, 0, at(2) - 16380, 0, None, None)),  # weight
+    ("ko_linear_mxfp4", (at(0), at(1), 0, at(2), at(3), at(4), 64, 64, 64, 0, at(3), 0, None, None)),
+    ("ko_linear_mxfp4", (at(0), at(1), 0, at(2), at(3), at(4), 64, 64, 64, 0, at(4) + 252, 0, None, None)),    # bias
+    ("ko_linear_quantize_mxfp4", (at(0), 0, 64, at(2), at(3), at(4), 4, 64, 64, 0, at(2), 0, None, 0, None, None)),
+    ("ko_linear_quantize_mxfp4", (at(0), 0, 64, at(2), at(3), at(4), 4, 64, 64, 0, at(3), 0, None, 0, None, None)),
+    ("ko_linear_quantize_mxfp4", (at(0), 0, 64, at(2), at(3), at(4), 4, 64, 64, 0, at(4), 0, None, 0, None, None)),
+    # 64 rows: a workspace of 4096 + 512 bytes, over x, out, the weight, its scales, the bias
+    *[("ko_linear_quantize_mxfp4", (at(0), 0, 64, at(2), at(3), at(4), 64, 64, 64, 0, at(5), 0, at(i) - 4592, 4608, None,
+                                    None)) for i in (0, 2, 3, 4, 5)],
+])
+def test_outputs_that_overlap_operands_are_refused(name, args):
+    with pytest.raises(ValueError, match="overlap"):
+        _lib.call(name, *args)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("ko_quantize_mx", (at(0), 0, 64, 64, 64, 0, at(0) + 16384, at(0) - 512, None)),
+    ("ko_dequantize_mx", (at(0), at(1), 0, 64, 64, at(0) + 4096, 0, None)),
+    ("ko_pack_weight_mxfp4", (at(0), 0, 64, 64, at(0) - 4096, at(0) + 16384, None)),
+    ("ko_linear_mxfp4", (at(0), at(1), 0, at(0), at(1), None, 64, 64, 64, 0, at(0) + 4096, 0, None, None)),   # x @ x^T
+    ("ko_linear_quantize_mxfp4", (at(0), 0, 64, at(2), at(3), at(4), 64, 64, 64, 0, at(5), 0, at(0) - 4608, 4608, None, None)),
+])
+def test_operands_that_only_touch_pass_the_checks(name, args):
+    if torch.cuda.is_available():
+        pytest.skip("would launch on made-up addresses")
+    with pytest.raises(_lib.KernelError):
+        _lib.call(name, *args)

@@ -57,3 +57,20 @@ def test_norm_output_in_place(cuda, rows, c, dtype, code):
         _lib.call("ko_residual_rmsnorm", a.data_ptr(), c, b.data_ptr(), c, None, None, gamma.data_ptr(), code, 1e-6, rows, c,
                   v_at.data_ptr(), y_at.data_ptr(), 0, None, None, torch.cuda.current_stream().cuda_stream)
         assert torch.equal(v_at, v) and torch.equal(y_at, y)
+
+
+def test_outputs_over_operands_are_refused(cuda):
+    """Through the Python entry points, which take `out` and `h_out` from the caller."""
+    x = torch.randn((64, 256), device=cuda)
+    pw = K.pack_weight_mxfp4(torch.randn((256, 32), device=cuda), torch.randn(32, device=cuda))
+    q = K.quantize_mx(x, "mxfp8")
+    over_codes = q.buf.view(torch.uint8).view(-1)[:64 * 32 * 4].view(torch.float32).view(64, 32)
+    over_x = x.view(-1)[256 * 64 - 2048:].view(64, 32)
+    for a, out in ((q, over_codes), (x, over_x)):
+        with pytest.raises(ValueError, match="overlap"):
+            K.linear_mxfp4(a, pw, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        K.linear_mxfp4(x[:1], pw, out=pw.bias.view(1, 32))
+    both = torch.ones(65 * 256, device=cuda)
+    with pytest.raises(ValueError, match="overlap"):
+        K.residual_rmsnorm(x, x, None, None, both[64 * 256:], 1e-6, h_out=both[256:].view(64, 256))
