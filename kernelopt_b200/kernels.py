@@ -717,7 +717,7 @@ def _rmsnorm(h, rows, ldh, o_ptr, ldo, bias, scale, gamma, eps, quantize, h_out_
 class PackedWeightMX:
     """A [K, N] weight as its transpose in mxfp4 (blocks along K), with its bias in fp32: linear_mxfp4's operand."""
 
-    __slots__ = ("mx", "k", "n", "bias", "ptrs", "status", "__weakref__")
+    __slots__ = ("mx", "k", "n", "_bias", "ptrs", "status", "__weakref__")
 
     def __init__(self, w, bias=None):
         if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype not in MX_DTYPES:
@@ -731,14 +731,32 @@ class PackedWeightMX:
         self.mx = MXTensor((self.n, self.k), "mxfp4", w.dtype, w.device)
         c, s = self.mx._ptrs()
         _call_on(w.device, "ko_pack_weight_mxfp4", w.data_ptr(), MX_DTYPES[w.dtype], self.k, self.n, c, s)
-        self.bias = None if bias is None else bias.detach().reshape(-1).to(torch.float32, copy=True)
+        self._bias = None if bias is None else bias.detach().reshape(-1).to(torch.float32, copy=True)
+        self._keep_addresses()
+
+    def _keep_addresses(self):
         # what every product with this weight passes: its addresses, and the device's status word, which never moves
-        self.ptrs = (c, s, _ptr(self.bias))
-        self.status = status_word(w.device).data_ptr()
+        self.ptrs = (*self.mx._ptrs(), _ptr(self._bias))
+        self.status = status_word(self.mx.device).data_ptr()
+
+    @property
+    def bias(self):
+        """The bias in fp32, or None. It cannot be replaced, only written to: products pass its address."""
+        return self._bias
+
+    def __reduce__(self):  # a copy, or what is read back from a file, has addresses of its own
+        return _packed_weight_mx, (self.mx, self.k, self.n, self._bias)
 
     def dequantize(self, dtype=torch.float32):
         """The [K, N] values that the packed weight stands for."""
         return self.mx.dequantize(dtype).t()
+
+
+def _packed_weight_mx(mx, k, n, bias):
+    pw = object.__new__(PackedWeightMX)
+    pw.mx, pw.k, pw.n, pw._bias = mx, k, n, bias
+    pw._keep_addresses()
+    return pw
 
 
 def pack_weight_mxfp4(w, bias=None) -> PackedWeightMX:

@@ -2,6 +2,10 @@
 formats holds against hand-computed values. No GPU needed."""
 from __future__ import annotations
 
+import copy
+import io
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -269,3 +273,28 @@ def test_operands_that_only_touch_pass_the_checks(name, args):
         pytest.skip("would launch on made-up addresses")
     with pytest.raises(_lib.KernelError):
         _lib.call(name, *args)
+
+
+@pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle", "save"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_copies_of_a_packed_weight_have_their_own_addresses(monkeypatch, how, bias):
+    """A product passes the addresses that the packed weight keeps, so a copy that kept the original's would read memory that
+    is freed with the original."""
+    monkeypatch.setattr(K, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    pw = K._packed_weight_mx(K.MXTensor((8, 64), "mxfp4", torch.bfloat16, "cpu"), 64, 8, torch.arange(8.0) if bias else None)
+    pw.mx.buf.fill_(7)
+    if how == "save":
+        f = io.BytesIO()
+        torch.save(pw, f)
+        f.seek(0)
+        other = torch.load(f, weights_only=False)
+    else:
+        other = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda p: pickle.loads(pickle.dumps(p))}[how](pw)
+    assert (other.k, other.n, other.mx.fmt, other.mx.shape, other.mx.dtype) == (64, 8, "mxfp4", (8, 64), torch.bfloat16)
+    assert torch.equal(other.mx.buf, pw.mx.buf)
+    assert other.ptrs == (*other.mx._ptrs(), other.bias.data_ptr() if bias else None)
+    assert (other.mx.buf.data_ptr() == pw.mx.buf.data_ptr()) == (how == "copy")
+    if bias:
+        assert torch.equal(other.bias, pw.bias)
+        with pytest.raises(AttributeError):
+            pw.bias = torch.zeros(8)

@@ -2,6 +2,8 @@
 and norms whose outputs take the place of their inputs."""
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
@@ -74,3 +76,15 @@ def test_outputs_over_operands_are_refused(cuda):
     both = torch.ones(65 * 256, device=cuda)
     with pytest.raises(ValueError, match="overlap"):
         K.residual_rmsnorm(x, x, None, None, both[64 * 256:], 1e-6, h_out=both[256:].view(64, 256))
+
+
+@pytest.mark.parametrize("m", [1, 40])
+def test_a_copied_weight_outlives_the_original(cuda, m):
+    g = torch.Generator(device=cuda).manual_seed(9)
+    x, w = torch.randn((m, 256), generator=g, device=cuda), torch.randn((256, 200), generator=g, device=cuda)
+    pw = K.pack_weight_mxfp4(w, torch.randn(200, generator=g, device=cuda))
+    want = K.linear_mxfp4(x, pw)
+    other = copy.deepcopy(pw)
+    pw.mx.buf.zero_()
+    pw.bias.zero_()
+    assert torch.equal(K.linear_mxfp4(x, other), want) and not K.linear_mxfp4(x, pw).any()
