@@ -952,10 +952,13 @@ int launch_slice(const Call& c) {
 
 // Which kernel, by the numbers of 256 x 128 tiles and of pipeline stages along K (mxfp4, bf16 outputs, us on B200):
 //   up to 64 rows, the slices: 48 x 8192 x 8192 in 9.9 against 14.8 with pairs.
-//   More rows and fewer tiles than stages, the slices too, for the pairs would leave most SMs idle behind a long K:
-//   300 x 4096 x 512 in 7.8 against 9.8; with more tiles, the pairs: 1200 x 4096 x 512 in 10.0 against 10.7 and
-//   1200 x 1024 x 1024 in 6.7 against 8.2. One tile of 128 rows reads the weight once, and there the slices keep a long K
-//   longer: 128 x 4096 x 4096 in 9.1 against 10.2.
+//   Up to 128 rows read the weight once, and a pair's tile would be half empty: the slices too, from 16 stages on (128 x 4096 x
+//   4096 in 8.8 against 10.2, 128 x 8192 x 20480 in 19.7 against 29.9; 128 x 2048 x 4096, eight stages, in 8.2 against 7.8).
+//   More rows, but no more tiles than stages, for the pairs would leave SMs idle behind a long K: the slices while a device
+//   with a CTA per 128 x 128 tile has SMs left to cut K for (300 x 4096 x 512 in 7.6 against 9.8; with more tiles than stages
+//   the pairs, 1200 x 4096 x 512 in 10.0 against 10.2, 1200 x 1024 x 1024 in 6.8 against 8.0). In mxfp8, 144 such tiles:
+//   1024 x 16384 x 2304 in 33 against 43, and 160, a second round of whole K: 1024 x 16384 x 2560 in 49 against 44, 768 x
+//   28672 x 8192 in 186 against 146.
 //   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.5 against 11.6) or K is so
 //   short that the epilogue counts: two stages (25664 x 512 x 1536 in 24.3 against 24.7), four with GELU (25664 x 1024 x
 //   1536 in 43 against 47; without, 34 against 30). Else 256 x 256, with less to load for a product (25664 x 2048 x 1536
@@ -967,7 +970,8 @@ int launch(const Call& c) {
   if (c.M <= 16) return launch_slice<F4, 16, T>(c);
   if (c.M <= 32) return launch_slice<F4, 32, T>(c);
   if (c.M <= 64) return launch_slice<F4, 64, T>(c);
-  if (tiles <= stages || (c.M <= 128 && stages >= 16)) return launch_slice<F4, 128, T>(c);
+  if (c.M <= 128 && stages >= 16) return launch_slice<F4, 128, T>(c);
+  if (tiles <= stages && (c.M + 127) / 128 * ((c.N + 127) / 128) <= c.info->sm_count) return launch_slice<F4, 128, T>(c);
   if (tiles <= c.info->sm_count / 2 || stages <= (c.act == KO_ACT_GELU ? 4 : 2)) return launch_pair<F4, 128, T>(c);
   return launch_pair<F4, 256, T>(c);
 }

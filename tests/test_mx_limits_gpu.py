@@ -88,3 +88,16 @@ def test_a_copied_weight_outlives_the_original(cuda, m):
     pw.mx.buf.zero_()
     pw.bias.zero_()
     assert torch.equal(K.linear_mxfp4(x, other), want) and not K.linear_mxfp4(x, pw).any()
+
+
+@pytest.mark.parametrize("m,n", [(2300, 1000), (2300, 1100), (290, 6200), (130, 10300)])
+@pytest.mark.parametrize("fmt,k", [("mxfp8", 10400), ("mxfp4", 20700)])
+def test_long_k_beside_many_tiles(cuda, fmt, k, m, n):
+    """No more tiles than stages of K, with 128 x 128 tiles for one round of the SMs and for more. Sums of products of -1, 0
+    and 1 are exact in every form of the product."""
+    g = torch.Generator(device=cuda).manual_seed(m + n)
+    x = torch.randint(-1, 2, (m, k), generator=g, device=cuda).to(torch.bfloat16)
+    w = torch.randint(-1, 2, (k, n), generator=g, device=cuda).to(torch.bfloat16)
+    got = K.linear_mxfp4(K.quantize_mx(x, fmt), K.pack_weight_mxfp4(w), out_dtype=torch.float32)
+    K.check_device_status(cuda)
+    assert torch.equal(got.double(), x.double() @ w.double())
