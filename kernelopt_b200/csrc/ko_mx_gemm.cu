@@ -959,10 +959,14 @@ int launch_slice(const Call& c) {
 //   the pairs, 1200 x 4096 x 512 in 10.0 against 10.2, 1200 x 1024 x 1024 in 6.8 against 8.0). In mxfp8, 144 such tiles:
 //   1024 x 16384 x 2304 in 33 against 43, and 160, a second round of whole K: 1024 x 16384 x 2560 in 49 against 44, 768 x
 //   28672 x 8192 in 186 against 146.
-//   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.5 against 11.6) or K is so
-//   short that the epilogue counts: two stages (25664 x 512 x 1536 in 24.3 against 24.7), four with GELU (25664 x 1024 x
-//   1536 in 43 against 47; without, 34 against 30). Else 256 x 256, with less to load for a product (25664 x 2048 x 1536
-//   with GELU in 53 against 61, 4096 x 8192 x 8192 in 98 against 141).
+//   Pairs with 256 x 128 tiles while these fill one round of the SMs (300 x 4096 x 4096 in 10.0 against 11.6), or where K is so
+//   short that the epilogue counts, over five shapes from 16384 x 1024 to 4096 x 8192 outputs. With GELU up to four stages: 1 to
+//   12 % faster than 256 x 256 (25664 x 1024 x 1536 in 45.6 against 49.2; with five 2 % slower to 6 % faster). Without it up to
+//   two: with 16-bit outputs 6 to 17 % faster at one stage (8192 x 256 x 4096 in 17.9 against 20.5), 4 % faster to 2 % slower at
+//   two and up to 11 % slower at three; with fp32 outputs, bound by their stores, 5 % faster to 9 % slower at one and two (4096 x
+//   512 x 8192 in 31.2 against 28.2), but 16 to 18 % faster where rows are not on 16 bytes (12000 x 512 x 2999 in 71 against 84).
+//   Else 256 x 256, with less to load for a product (25664 x 2048 x 1536 with GELU in 56 against 65, 4096 x 8192 x 8192 in 99
+//   against 145).
 template <bool F4, typename T>
 int launch(const Call& c) {
   const int64_t tiles = ((c.M + 255) / 256) * ((c.N + 127) / 128);
