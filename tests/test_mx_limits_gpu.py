@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import copy
 
+import numpy as np
 import pytest
 import torch
 
@@ -101,3 +102,23 @@ def test_long_k_beside_many_tiles(cuda, fmt, k, m, n):
     got = K.linear_mxfp4(K.quantize_mx(x, fmt), K.pack_weight_mxfp4(w), out_dtype=torch.float32)
     K.check_device_status(cuda)
     assert torch.equal(got.double(), x.double() @ w.double())
+
+
+@pytest.mark.parametrize("m", [1, 20, 100])
+def test_gelu_below_zero_keeps_its_digits(cuda, m):
+    """Relative to the result, reached through the bias of a product of zeros. On [-6, 0) the kernel's erfc is a fit within 3e-5
+    of itself times an exponential whose argument, up to 26, is off by two roundings: 26 * 2^-23; the products and the sum
+    add less than 2^-20. Beyond -6 it is the value at 6 times that exponential, so too small by 1 - 6 g(6) / (|v| g(|v|))."""
+    from scipy.special import erfc
+
+    v = np.concatenate([-np.geomspace(1e-6, 6, 400), -np.linspace(6.01, 13.1, 400)]).astype(np.float32)
+    pw = K.pack_weight_mxfp4(torch.ones((64, 800), device=cuda), torch.from_numpy(v).to(cuda))
+    got = K.linear_mxfp4(torch.zeros((m, 64), device=cuda), pw, "gelu")
+    K.check_device_status(cuda)
+    assert bool((got == got[0]).all())
+    v = v.astype(np.float64)
+    off = got[0].double().cpu().numpy() / (0.5 * v * erfc(-v / np.sqrt(2.0))) - 1
+    assert np.abs(off[:400]).max() <= 3e-5 + 26 * 2.0 ** -23 + 2.0 ** -20
+    at = lambda x: x * erfc(x / np.sqrt(2.0)) / 2 * np.exp(x * x / 2)  # noqa: E731  |v| g(|v|)
+    small = 1 - at(6.0) / at(-v[400:])
+    assert small[-1] < 0.026 and np.abs(off[400:] + small).max() <= 3e-5 + 124 * 2.0 ** -23 + 2.0 ** -20
