@@ -11,6 +11,8 @@ import torch
 from kernelopt_b200 import _lib
 from kernelopt_b200 import kernels as K
 
+import test_mx_gpu as T
+
 pytestmark = pytest.mark.gpu
 
 
@@ -122,3 +124,49 @@ def test_gelu_below_zero_keeps_its_digits(cuda, m):
     at = lambda x: x * erfc(x / np.sqrt(2.0)) / 2 * np.exp(x * x / 2)  # noqa: E731  |v| g(|v|)
     small = 1 - at(6.0) / at(-v[400:])
     assert small[-1] < 0.026 and np.abs(off[400:] + small).max() <= 3e-5 + 124 * 2.0 ** -23 + 2.0 ** -20
+
+
+@pytest.mark.parametrize("m", [1, 40, 300, 700])
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+@pytest.mark.parametrize("ex,ew", [(-126, 126), (126, -126), (127, -126), (-126, 127), (-127, 100), (100, -127), (-133, 60)])
+def test_block_scales_at_both_ends(cuda, fmt, m, ex, ew):
+    """Products of blocks whose scale bytes are the lowest (0) or near the highest (252 and 246), down to subnormal elements:
+    -1, 0 and 1 times 2^ex and 2^ew, whose sums are exact."""
+    k, n = 640, 520
+    g = torch.Generator(device=cuda).manual_seed(m)
+    x = torch.randint(-1, 2, (m, k), generator=g, device=cuda).double()
+    w = torch.randint(-1, 2, (k, n), generator=g, device=cuda).double()
+    a, b = ((t * 2.0 ** e).to(torch.float32) for t, e in ((x, ex), (w, ew)))
+    least = -128 if fmt == "mxfp4" else -136          # the smallest element beside the scale 2^-127
+    q, pw = K.quantize_mx(a, fmt), K.pack_weight_mxfp4(b)
+    assert int(q.scales.view(torch.uint8).max()) == max(127 + ex - (2 if fmt == "mxfp4" else 8), 0)
+    want = (x @ w) * 2.0 ** (ex + ew) if ex >= least else torch.zeros((m, n), dtype=torch.float64, device=cuda)
+    assert torch.equal(K.linear_mxfp4(q, pw, out_dtype=torch.float32).double(), want)
+    if fmt == "mxfp4":
+        assert torch.equal(K.linear_mxfp4(a, pw).double(), want)
+    K.check_device_status(cuda)
+
+
+@pytest.mark.parametrize("m", [1, 40, 700])
+def test_a_product_over_the_range_is_infinite(cuda, m):
+    x = torch.zeros((m, 256), device=cuda)
+    x[:, 7] = 2.0 ** 127
+    w = torch.zeros((256, 16), device=cuda)
+    w[7, :8], w[7, 8:] = 2.0 ** 3, -2.0 ** 3
+    got = K.linear_mxfp4(x, K.pack_weight_mxfp4(w))
+    assert bool((got[:, :8] == float("inf")).all()) and bool((got[:, 8:] == -float("inf")).all())
+
+
+@pytest.mark.parametrize("out", [None, "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", T.DTYPES)
+@pytest.mark.parametrize("rows,c,affine", [(3, 16385, True), (2, 20001, False), (2, 32767, True)])
+def test_norm_of_the_widest_rows_element_by_element(cuda, rows, c, affine, dtype, out):
+    args = T.norm_inputs(rows, c, rows + c, dtype, cuda, affine)
+    v, dv, y, dy = T.norm_oracle(*args, 1e-6)
+    got_v, got_y = K.residual_rmsnorm(*args, 1e-6, quantize=out)
+    half, tiny = T.HALF[dtype], T.TINY[dtype]
+    assert (np.abs(T.np64(got_v) - v) <= dv + half * (np.abs(v) + dv) + tiny).all(), "v"
+    if out is None:
+        assert (np.abs(T.np64(got_y) - y) <= dy + half * (np.abs(y) + dy) + tiny).all(), "y"
+    else:
+        T.check_norm_quantized(got_y, y, dy)
