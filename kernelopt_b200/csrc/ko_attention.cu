@@ -166,19 +166,6 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128_32b(uint32_t addr) {
   return d;
 }
 
-// tcgen05 of a CTA pair (cta_group::2): every tcgen05 operation of the kernel names the pair. The allocation is made
-// by warp 0 of both CTAs with the same destination slot.
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst_smem)),
-               "r"(ncols)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish_pair() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
 // D (+)= A B over the pair, A and B from shared memory (elected lane of the calling warp).
 __device__ __forceinline__ void mma_pair_tf32_w(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                                 uint32_t accumulate) {
@@ -197,15 +184,6 @@ __device__ __forceinline__ void mma_pair_tf32_ts_w(uint32_t d_tmem, uint32_t a_t
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrive once on `bar` in both CTAs of the pair when every MMA issued so far by this thread has completed.
-__device__ __forceinline__ void mma_commit_pair_w(uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t.reg .b16 mask;\n\tmov.b16 mask, 3;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], mask;\n\t}"
-      ::"r"(smem_addr(bar))
-      : "memory");
-}
-
 // The part of v below its tf32 truncation: v - (v with the low 13 mantissa bits cleared), exact in fp32. P is kept
 // as v in the P_hi slot (the tensor core reads a tf32 operand from the top 19 bits of the word, i.e. truncates)
 // and this tail in P_lo, so P = P_hi + P_lo exactly before the MMA truncates P_lo (an error below 2^-20 P).
