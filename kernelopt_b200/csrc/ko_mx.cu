@@ -156,12 +156,17 @@ __global__ void __launch_bounds__(kThreads) pack_weight_kernel(const T* __restri
 // registers from the load to the store, so h and o are read once; the sum of squares is a shuffle tree and, for rows of
 // more than a warp, one exchange through shared memory, both in a fixed order. Four lanes hold a block of 32 and sixteen
 // the 128 elements of a scale word, so a quantised block costs two shuffles and its scales are stored a word at a time.
-// Bound by HBM: 16384 x 8192 bf16 to mxfp8 in 153 us (6.2 TB/s; 68 % of the issue slots), 25664 x 384 fp32 in 20 to 24 us.
+// Bound by HBM: 16384 x 8192 bf16 to mxfp8 in 154 us (6.2 TB/s; 68 % of the issue slots), 25664 x 384 fp32 with bias and scale in
+// 25.6 us (5.0 TB/s), 23.2 without. Rows that are not whole groups of eight are read and written element by element, neighbouring
+// lanes 16 or 32 bytes apart, and bound by that: 16384 x 1001 to mxfp8 in 81 us from fp32 and 57 from bf16 (2.7 and 2.0 TB/s),
+// as values in 158 and 86.
 // OUT: -1 writes y in the input's type, else the MX format.
 // ---------------------------------------------------------------------------------------------------------
 // 1 / sqrt(x) as the sum of two fp32 numbers: the special-function value r and one Newton step's correction, r (1 - x r^2)
-// / 2, with r^2 kept exactly. y then has the roundings of v * gamma and of the product only, which decides how many 8-bit
-// codes next to a border come out on the other side. Where r^2 could leave the range, r is the rounded value alone.
+// / 2, with r^2 kept exactly. y then has the roundings of v * gamma and of the product, and none of r: 5.7e-8 from the exact
+// values in the 2-norm (25664 x 384 fp32), as a division in fp32 has it, 6.2e-8 with the rounded 1 / sqrt(x) alone. Most shapes
+// take the same time without it, 16384 x 4096 bf16 to mxfp8 76.8 us instead of 79.9. About one 8-bit code in a million, next
+// to a border, comes out on its other side either way. Where r^2 could leave the range, r is the rounded value alone.
 __device__ __forceinline__ float2 inverse_root(float x) {
   if (!(x > 1e-30f && x < 1e30f)) return make_float2(1.0f / sqrtf(x), 0.f);
   const float r = rsqrtf(x), t = r * r;
@@ -337,7 +342,8 @@ int pick_norm(const NormArgs& a, cudaStream_t s) {
   // thread), with no more groups than the row has. Then two groups of eight to a thread: 16384 x 4096 in 127 us fp32 and
   // 78 us bf16, 130 and 80 with half the threads, 127 and 92 with twice as many; one row of 4096 in 2.4 us, 2.8 and 2.4.
   // From 8192 on the threads of a block bound it: 8192 x 16384 bf16 in 148 us with 512 threads and four groups, 212 with
-  // 1024 and two.
+  // 1024 and two. 1024 threads leave 64 registers each, and rows over 16384 that are read element by element do not fit: 16-bit
+  // ones spill 60 to 92 bytes, fp32 ones 4.
   if (a.C <= 128) return launch_norm<T, OUT, VEC, 16, 1>(a, s);
   if (a.C <= 256) return launch_norm<T, OUT, VEC, 16, 2>(a, s);
   if (a.C <= 384) return launch_norm<T, OUT, VEC, 16, 3>(a, s);
