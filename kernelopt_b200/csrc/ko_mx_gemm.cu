@@ -117,19 +117,21 @@ __device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 // GELU of two values: v Phi(v) = max(v, 0) - |v| q with q = erfc(|v| / sqrt 2) / 2 = exp(-v^2 / 2) g(|v|). g is smooth
-// on [0, 6] (it falls from 1/2 to 0.065), so a polynomial of degree 12 in |v| / 3 - 1 has it, fitted by least squares at
-// Chebyshev nodes: there q is within 3e-5 of itself, so that small negative results keep their digits, and |v| q within 8e-8.
-// Beyond 6, |v| g(|v|) stays at 6 g(6) = 0.389, on its way to 1 / sqrt(2 pi) = 0.399: results that are below 6e-9 there come
-// out too small in magnitude, by 0.7 % at -7, 1.4 % at -9, 2 % at -13 and less than 2.6 % anywhere, and 0 below -13.2, where
-// the exponential leaves the normal fp32 numbers. NaN stays NaN, and GELU(-inf) is 0, its limit.
+// on [0, 6] (it falls from 1/2 to 0.065), so a polynomial of degree 12 in |v| / 3 - 1 has it. Its fit is minimax (Lawson's
+// weights) in what counts of g's error: |v| q is within 7e-8, for small |v| within 2.4e-7 |v|, so that small results keep their
+// digits, and q within 2.4e-5 of itself, so that those on the negative side do. Least squares alone, with the same error of g
+// everywhere, had 2.4e-6 |v| next to zero. Beyond 6, |v| g(|v|) stays at 6 g(6) = 0.389, on its way to 1 / sqrt(2 pi) = 0.399:
+// results that are below 6e-9 there come out too small in magnitude, by 0.7 % at -7, 1.4 % at -9, 2 % at -13 and less than 2.6 %
+// anywhere, and 0 below -13.2, where the exponential leaves the normal fp32 numbers. NaN stays NaN, and GELU(-inf) is 0, its
+// limit.
 // It costs one special-function instruction, and all else but the ends is packed: 25664 x 384 x 1536 with fp32 outputs takes
 // 34 us without an activation and 41 with this one. A&S 7.1.26 as the fp32-grade GEMM has it (two special-function
 // instructions, not packed) added 30 us to the same product at an earlier state of the epilogue.
 __device__ __forceinline__ void gelu_pair(float& a, float& b) {
-  constexpr float g[13] = {-0.12151393294334412f, 0.10320935398340225f, -0.08236773312091827f, 0.062280356884002686f,
-                           -0.04567015543580055f, 0.03141380101442337f, -0.01772490330040455f, 0.013943932950496674f,
-                           -0.015077504329383373f, 0.0027330496814101934f, 0.004123609978705645f, 0.004027877002954483f,
-                           -0.004158561583608389f};
+  constexpr float g[13] = {-0.12151453644037247f, 0.10321106761693954f, -0.0823381170630455f, 0.06228569149971008f,
+                           -0.04591979831457138f, 0.03130459412932396f, -0.01686754636466503f, 0.01429088693112135f,
+                           -0.01651555486023426f, 0.0023183149751275778f, 0.005299349781125784f, 0.0041989353485405445f,
+                           -0.004534068051725626f};
   const uint64_t ax = pack_f2(fminf(fabsf(a), 6.f), fminf(fabsf(b), 6.f));
   const uint64_t s = fma_f2(ax, pack_f2(1.f / 3.f, 1.f / 3.f), pack_f2(-1.f, -1.f));
   uint64_t p = pack_f2(g[12], g[12]);

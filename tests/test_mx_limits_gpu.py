@@ -170,3 +170,23 @@ def test_norm_of_the_widest_rows_element_by_element(cuda, rows, c, affine, dtype
         assert (np.abs(T.np64(got_y) - y) <= dy + half * (np.abs(y) + dy) + tiny).all(), "y"
     else:
         T.check_norm_quantized(got_y, y, dy)
+
+
+@pytest.mark.parametrize("m", [1, 20, 100])
+def test_gelu_next_to_zero_keeps_its_digits(cuda, m):
+    """Relative to the result on both sides of zero. There q = erfc / 2 is near 1/2, so an error of |v| times 2.4e-7 in |v| q
+    is one of 4.8e-7 at most of the result, at |v| = 1/2 on the negative side of 7.8e-7; the polynomial's twelve steps, of
+    partial sums below 0.6, add 12 * 0.6 * 2^-24 to q and the other five roundings 2^-24 of it each, both doubled at zero
+    and over 0.31 at |v| = 1/2."""
+    from scipy.special import erfc
+
+    v = np.geomspace(1e-30, 0.5, 400)
+    v = np.concatenate([v, -v]).astype(np.float32)
+    pw = K.pack_weight_mxfp4(torch.ones((64, 800), device=cuda), torch.from_numpy(v).to(cuda))
+    got = K.linear_mxfp4(torch.zeros((m, 64), device=cuda), pw, "gelu")
+    K.check_device_status(cuda)
+    assert bool((got == got[0]).all())
+    v = v.astype(np.float64)
+    off = got[0].double().cpu().numpy() / (0.5 * v * erfc(-v / np.sqrt(2.0))) - 1
+    q = np.minimum(0.5 * erfc(np.abs(v) / np.sqrt(2.0)), 0.5 * erfc(-v / np.sqrt(2.0)))
+    assert (np.abs(off) <= (2.4e-7 + (12 * 0.6 + 5) * 2.0 ** -24) / q).all(), np.abs(off).max()
