@@ -511,7 +511,7 @@ extern "C" int ko_residual_rmsnorm(const void* h, int64_t ldh, const void* o, in
   // fine. Every other overlap of an output is not: with another row, with the vectors, that all rows read, or with another
   // output.
   const int64_t es = dtype_size(dtype), out_bytes = rows * C * es;
-  const Range hs = span_of(h, rows, ldh, C, es), os = span_of(o, rows, ldo, C, es);
+  const Range hs = span_of(h, rows, ldh, C, es), os = span_of(o, rows, o ? ldo : C, C, es);
   const Range vs[] = {{bias, C * es}, {scale, C * es}, {gamma, C * es}};
   const Range ho = {h_out, out_bytes}, yo = {y, out_bytes}, co = {codes, y ? 0 : ko_mx_codes_bytes(rows, C, fmt)},
               so = {scales, y ? 0 : ko_mx_scales_bytes(rows, C)};

@@ -17,7 +17,7 @@ LayerNorm epilogue (`linear_residual_layernorm`) and the implicit 3x3 convolutio
 `select_queries` and `deform_prep`.
 And a microscaled (OCP MX) path, which the reference has no counterpart of: `quantize_mx`, `residual_rmsnorm` /
 `rmsnorm` with an mxfp8 or mxfp4 output, and `pack_weight_mxfp4` / `linear_mxfp4`. These take float32, bfloat16 and
-float16, any width and any even row pitch (column slices), and launch on the device of their tensors.
+float16, any width and rows that are evenly spaced (column slices), and launch on the device of their tensors.
 """
 from __future__ import annotations
 
@@ -663,7 +663,7 @@ class MXTensor:
 
 
 def quantize_mx(x, fmt="mxfp4") -> MXTensor:
-    """x [..., K] float32, bfloat16 or float16 (any even row pitch) in a microscaled format: per block of 32 along K the
+    """x [..., K] float32, bfloat16 or float16 (evenly spaced rows) in a microscaled format: per block of 32 along K the
     scale 2^(floor(log2(max |x|)) - 2) (mxfp4; - 8 for mxfp8), held to 2^-127 or above, and x / scale to the nearest
     element, ties to even, saturating. A block holding a NaN or an infinity becomes NaN."""
     rows, pitch = _rows(x, "x")
@@ -676,7 +676,7 @@ def quantize_mx(x, fmt="mxfp4") -> MXTensor:
 def residual_rmsnorm(h, o, bias, scale, gamma, eps, quantize=None, h_out=None):
     """Returns (v, y) with v = h + (o + bias) * scale and y = v / sqrt(mean(v^2) + eps) * gamma over the last dimension
     (width <= 32768), both computed in fp32: residual_layernorm's arguments for a model that normalises by the root
-    mean square. h and o: [..., C] float32, bfloat16 or float16 (any even row pitch); bias and scale [C] or None (0 / 1);
+    mean square. h and o: [..., C] float32, bfloat16 or float16 (evenly spaced rows); bias and scale [C] or None (0 / 1);
     gamma [C]; all of one type. v is returned in that type, in h_out where given ([..., C] contiguous; h or o itself, or
     apart from both). y has that type too, or is with quantize "mxfp8" / "mxfp4" an MXTensor, quantised from fp32 in the
     same pass."""
@@ -686,7 +686,8 @@ def residual_rmsnorm(h, o, bias, scale, gamma, eps, quantize=None, h_out=None):
     _, ldo = _rows(o, "o", h.dtype, h.device)
     if h_out is None:
         h_out = torch.empty_like(h) if h.is_contiguous() else _dense(h.shape, h.dtype, h.device)
-    elif not isinstance(h_out, torch.Tensor) or h_out.shape != h.shape or h_out.dtype != h.dtype or h_out.device != h.device or not h_out.is_contiguous():
+    elif (not isinstance(h_out, torch.Tensor) or h_out.shape != h.shape or h_out.dtype != h.dtype
+          or h_out.device != h.device or not h_out.is_contiguous()):
         raise ValueError("h_out must be contiguous, of h's shape, type and device")
     return h_out, _rmsnorm(h, rows, ldh, o.data_ptr(), ldo, bias, scale, gamma, eps, quantize, h_out.data_ptr())
 
@@ -760,7 +761,8 @@ def _packed_weight_mx(mx, k, n, bias):
 
 
 def pack_weight_mxfp4(w, bias=None) -> PackedWeightMX:
-    """Quantises w [K, N] (x @ W) once for linear_mxfp4. The bias is copied."""
+    """Quantises w [K, N] (x @ W) once for linear_mxfp4, on the current stream of w's device: a product on another stream has
+    to be ordered behind it. The bias is copied."""
     return PackedWeightMX(w, bias)
 
 
@@ -768,7 +770,8 @@ def linear_mxfp4(x, pw: PackedWeightMX, act=None, out_dtype=None, out=None):
     """act(x @ W + bias) with W in mxfp4, on the block-scaled tensor-core products with fp32 accumulation. x: an
     MXTensor [..., K] (mxfp8 or mxfp4), or a float32 / bfloat16 / float16 tensor, which is quantised to mxfp4 (up to 16
     rows inside the product's kernel, more in a pass before it). act None, 'gelu' or 'relu'. The output [..., N] is rounded
-    once, to out_dtype (x's type by default). out, where given, is contiguous and does not overlap x."""
+    once, to out_dtype (x's type by default). out, where given, is contiguous and overlaps neither x nor the weight or its
+    bias. A row's sum is taken in an order that the sizes decide (rows, K and N), the same every time."""
     if act not in ACTS:
         raise ValueError(f"act must be one of {list(ACTS)}")
     wdev = pw.mx.buf.device

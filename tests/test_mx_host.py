@@ -218,6 +218,7 @@ def test_norm_outputs_that_overlap_are_refused(args):
 @pytest.mark.parametrize("args", [
     norm_call(), norm_call(y=A), norm_call(y=9 * A), norm_call(h_out=A, y=9 * A), norm_call(h_out=9 * A, y=A),
     norm_call(o=A, h_out=None, y=A), norm_call(rows=1, ldh=72, y=A), norm_call(o=None, ldo=0, h_out=None, y=A),
+    norm_call(o=None, ldo=1 << 62),
     norm_call(y=A + 4 * ROW), norm_call(y=A - 4 * ROW), norm_call(y=11 * A + 4 * ROW),
     norm_call(y=None, codes=14 * A, scales=14 * A + 256), norm_call(y=None, fmt=1, codes=A + 4 * ROW, scales=A + 4 * ROW + 512),
 ])
